@@ -52,6 +52,7 @@ typedef enum llmoc_status {
 
 enum { LLMOC_SCHEME_GPTQ_ASYM = 1, LLMOC_SCHEME_AWQ_SYM = 2 };
 enum { LLMOC_ROUTER_SOFTMAX = 0, LLMOC_ROUTER_SIGMOID_BIAS = 1 };
+enum { LLMOC_DTYPE_F32 = 0, LLMOC_DTYPE_BF16 = 1 };
 
 /* Layout-identical to qlwc::Int4View (src/weights/qlwc_store.h:17-27). */
 typedef struct llmoc_int4_view {
@@ -308,6 +309,141 @@ LLMOC_API size_t llmoc_moe_noalloc_capacity(void);
  * up (its outputs are then not valid), LLMOC_OK otherwise. */
 LLMOC_API llmoc_status llmoc_moe_noalloc_status(const llmoc_moe_layer* layer, int T, void* stream);
 
+/* ----------------------------------------- operators around the MoE layer
+ *
+ * What a decode step runs beside the MoE layer, on the device and asynchronous
+ * on `stream`: dense INT4 products (attention projections, dense FFNs, the
+ * output head), the norms, gate and residual between blocks, and a step of
+ * beam search with the reordering of the beams' states.  Each call works on
+ * `device` (or its handle's device) whatever the current one is, restores the
+ * current device, allocates nothing, and can be captured into a CUDA graph.
+ * `stream` must belong to that device.  Row strides (ld*) count elements. */
+
+enum { LLMOC_NORM_NONE = 0, LLMOC_NORM_RMS = 1, LLMOC_NORM_LAYER = 2 };
+enum { LLMOC_ACT_NONE = 0, LLMOC_ACT_SIGMOID = 1 };
+
+/* Dense INT4 weights resident on one device: the device-resident, asynchronous
+ * form of hal::cuda::try_gemm_int4 / _batch / _multi (cuda_backend.h:165-172),
+ * which take host fp32 rows and synchronise.  n_views projections that share
+ * their input (e.g. query, key and value) are stacked into one product of
+ * M = sum of their rows; they agree in K, group size, scheme and zero point, and
+ * every one but the last has a multiple of 16 rows.  K and the group size are
+ * multiples of 32 (LLMOC_ERR_UNSUPPORTED otherwise); M is any.  on_device: the
+ * views point to memory of `device`, complete when the call is made.  The
+ * views' buffers are not kept. */
+typedef struct llmoc_int4_linear llmoc_int4_linear;
+LLMOC_API llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views, int device, int on_device,
+                                                llmoc_int4_linear** out);
+LLMOC_API void llmoc_int4_linear_destroy(llmoc_int4_linear* linear);
+/* Bytes of resident weights one product streams (packed q + fp16 scales / zeros, with the padding to 16 rows x 64 k). */
+LLMOC_API size_t llmoc_int4_linear_weight_bytes(const llmoc_int4_linear* linear);
+/* Y[t, m] = sum_k W[m, k] X[t, k] (+ R[t, m]), t < T, one rounding to y_dtype
+ * (LLMOC_DTYPE_*): products of bf16 activations with exact integers, group
+ * sums and their scaled sum in fp32, a fixed order of summation.  X, R bf16; R
+ * may be null, and may be Y itself (bf16, ldr = ldy).  X overlaps neither R
+ * nor Y.  T = 0 does nothing. */
+LLMOC_API llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* linear, const uint16_t* X, int64_t ldx, int T,
+                                                 const uint16_t* R, int64_t ldr, void* Y, int64_t ldy, int y_dtype,
+                                                 void* stream);
+
+/* Between two blocks of a decoder (the reference's rmsnorm_w16 and vec_add
+ * launches, src/hal/cuda_backend.cpp, in one pass over the rows):
+ *     u  = post(block)
+ *     r  = residual_scale * residual + block_scale * act(gate) * u
+ *     n  = pre(r)
+ * with RMS norm x / sqrt(mean(x^2) + eps) * (weight + weight_offset) (+ bias)
+ * or layer norm, the same of x - mean(x).  fp32 inside; residual_out is r
+ * rounded to the residual's type, norm_out is n of the unrounded r. */
+typedef struct llmoc_norm_desc {
+  int32_t hidden;            /* H <= 16384 */
+  int32_t post, pre;         /* LLMOC_NORM_* */
+  int32_t weight_dtype;      /* LLMOC_DTYPE_* of the four vectors below */
+  const void* post_weight;   /* [H] or null (ones; weight_offset not added) */
+  const void* post_bias;     /* [H] or null */
+  const void* pre_weight;
+  const void* pre_bias;
+  float weight_offset;       /* 0, or 1 for weights stored around zero */
+  float eps;                 /* > 0 */
+  float block_scale, residual_scale;
+  int32_t gate_act;          /* LLMOC_ACT_* */
+} llmoc_norm_desc;
+typedef struct llmoc_norm_io {
+  const void* block;         /* [T][H] or null: no block, r = residual_scale * residual */
+  int64_t ld_block;
+  const void* residual;      /* [T][H] or null: no residual */
+  int64_t ld_residual;
+  void* residual_out;        /* [T][H] or null; may be `residual` or `block` itself (same type and stride) */
+  int64_t ld_residual_out;
+  void* norm_out;            /* [T][H] or null; may be `block` or `residual` itself (same type and stride),
+                                but not residual_out */
+  int64_t ld_norm_out;
+  const void* gate;          /* or null; element (t, h) at t * gate_row_stride + h * gate_col_stride */
+  int64_t gate_row_stride;   /* >= 0; 0: the same for every token */
+  int64_t gate_col_stride;   /* 0 (one per token) or 1 */
+  int32_t block_dtype, residual_dtype, norm_dtype, gate_dtype; /* LLMOC_DTYPE_* (residual_dtype: in and out) */
+} llmoc_norm_io;
+LLMOC_API llmoc_status llmoc_norm_residual(const llmoc_norm_desc* desc, const llmoc_norm_io* io, int T, int device,
+                                           void* stream);
+
+/* A decoder's whole MoE block on its residual stream (bf16 [T, hidden]):
+ *     x = in(residual);  b = MoE(x);
+ *     (residual_out, norm_out) = llmoc_norm_residual(out, {b, residual, gate})
+ * `in` uses its pre norm only (its block, gate and scales are not applied);
+ * out is the block's own post norm, scales and next norm; io gives residual,
+ * residual_out, norm_out and gate (block is taken from the MoE layer, and the
+ * dtypes of residual and norm_out must be bf16).  residual_out may be residual. */
+LLMOC_API size_t llmoc_moe_block_workspace_bytes(const llmoc_moe_layer* layer, int max_tokens);
+LLMOC_API llmoc_status llmoc_moe_forward_block(const llmoc_moe_layer* layer, const llmoc_norm_desc* in,
+                                               const llmoc_norm_desc* out, const llmoc_norm_io* io, int T,
+                                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* One step of beam search (the sampling next to llmoc_try_gemm_int4_argmax;
+ * no reference counterpart).  logits [batch * beams][ld >= vocab], bf16 or
+ * fp32; candidate (w, v) of sequence b has the value
+ *     scores[b][w] + logit - log sum exp(logits of the beam),
+ * and the n_out best over all beams and tokens, ordered by value, then beam,
+ * then token, are written: parent (the beam), token, out_scores, all
+ * [batch][n_out].  Non-finite logits are masked: their tokens are no
+ * candidates and add nothing to the sum.  A beam whose score is not finite has
+ * no candidates (e.g. all but the first of a sequence's first step).  A beam
+ * with finished[b][w] != 0 has one: (eos_token, its score unchanged).  Where
+ * fewer candidates exist, the rest is parent = token = -1, score = -inf.
+ * finished_out[b][k] = the parent is finished, or the token is eos_token.
+ * finished and finished_out may be null; finished needs an eos_token in
+ * [0, vocab), else it may be -1.  Outputs may not overlap inputs.
+ * beams, n_out <= 128. */
+typedef struct llmoc_beam_desc {
+  int32_t batch, beams, vocab, n_out, eos_token;
+} llmoc_beam_desc;
+LLMOC_API size_t llmoc_beam_workspace_bytes(const llmoc_beam_desc* desc);
+LLMOC_API llmoc_status llmoc_beam_select(const llmoc_beam_desc* desc, const void* logits, int64_t ld, int logits_dtype,
+                                         const float* scores, const uint8_t* finished, int32_t* parent, int32_t* token,
+                                         float* out_scores, uint8_t* finished_out, void* workspace,
+                                         size_t workspace_bytes, int device, void* stream);
+
+/* The beams' states in the chosen order: row k of sequence b of dst becomes
+ * row parent[b][k] of sequence b of src, for n_tensors tensors at once (e.g.
+ * every layer's cache).  A row is n_seg segments of seg_bytes, seg_stride bytes
+ * apart; row w of sequence b of src starts at (b * beams + w) * src_stride
+ * bytes, of dst at (b * n_out + k) * dst_stride.  So a cache [rows][heads][max
+ * length][width] is moved up to its used length with n_seg = heads, and a
+ * time-major one with n_seg = length.  Rows whose parent lies outside
+ * [0, beams) (e.g. -1) are left as they were, as is what lies between
+ * segments.  A tensor may be reordered in place (dst == src, same strides,
+ * n_out == beams): rows that stay are not touched.  Otherwise dst overlaps no
+ * src (LLMOC_ERR_INVALID).  n_out <= 64.  The tensors' addresses are taken
+ * when the call is made; parent is read on the device. */
+typedef struct llmoc_reorder_tensor {
+  const void* src;
+  void* dst;
+  int64_t src_stride, dst_stride; /* bytes between rows */
+  int64_t seg_stride;             /* bytes between a row's segments (any when n_seg = 1) */
+  int64_t seg_bytes;
+  int32_t n_seg;
+} llmoc_reorder_tensor;
+LLMOC_API llmoc_status llmoc_beam_reorder(const llmoc_reorder_tensor* tensors, int n_tensors, const int32_t* parent,
+                                          int batch, int beams, int n_out, int device, void* stream);
+
 /* ------------------------------------------------- expert parallelism (EP)
  * The reference gives only the contracts: expert e is owned by rank
  * e % world (DeviceMesh::owner_rank with EpShard::kMod,
@@ -425,7 +561,6 @@ LLMOC_API llmoc_status llmoc_ep_p2p_finish(const llmoc_moe_layer* shard, llmoc_e
  * the second waits and consumes) so that several ranks' objects can share
  * one stream in one process; the op calls are start + finish. */
 enum { LLMOC_COLL_ALLTOALL = 0, LLMOC_COLL_ALLREDUCE_SUM = 1, LLMOC_COLL_BROADCAST = 2 };
-enum { LLMOC_DTYPE_F32 = 0, LLMOC_DTYPE_BF16 = 1 };
 typedef struct llmoc_collective llmoc_collective;
 /* Allocates this rank's buffer (2 x world x max_bytes of staging) and writes
  * its IPC handle (llmoc_ep_ipc_handle_bytes() bytes; may be null for

@@ -1,0 +1,103 @@
+// ops.cuh — argument structs and launchers of the operators around the MoE
+// layer: dense INT4 products (linear.cu), residual norms (norm.cu), beam
+// selection and state reordering (beam.cu).  Host side: ops_runtime.cu.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+#include <string>
+
+#include "common.cuh"
+
+namespace llmoc {
+
+// ---- linear.cu
+struct LinArgs {
+  const uint4* q;   // fragment order (common.cuh)
+  const __half2* s; // [Mt][ng][8]: the scales of rows g and g + 8 of a tile side by side
+  const __half2* z; // GPTQ zeros, same layout, or null
+  int M, K, Kc, ng, gs;
+  int mt;           // 16-row tiles
+  int zp;
+  const __nv_bfloat16* X;
+  long long ldx;
+  int T;
+  const __nv_bfloat16* R;  // [T][M] added before the rounding, or null
+  long long ldr;
+  void* Y;
+  long long ldy;
+  int y_f32;
+  int x_vec;        // X rows readable by 16-byte loads
+  int ks;           // warps of a CTA that split K
+  int ntb;          // token blocks
+};
+// [n][16] fp16 (rows of a tile) -> the same 16 values as pairs (g, g + 8), in place
+cudaError_t launch_pair_rows(uint16_t* s, size_t n, cudaStream_t st);
+cudaError_t launch_linear(const LinArgs& a, bool awq, cudaStream_t st);
+
+// ---- norm.cu
+struct NormArgs {
+  const void* block;
+  const void* res;
+  void* res_out;
+  void* out;
+  const void* post_w;
+  const void* post_b;
+  const void* pre_w;
+  const void* pre_b;
+  const void* gate;
+  long long ld_block, ld_res, ld_res_out, ld_out, gate_row, gate_col;
+  int T, H;
+  int post, pre;  // LLMOC_NORM_*
+  int block_f32, res_f32, out_f32, w_f32, gate_f32, gate_sigmoid;
+  float w_off, eps, block_scale, res_scale;
+  int vec;  // every row of every operand readable by 16-byte loads
+};
+constexpr int kNormMaxH = 16384;
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t st);
+
+// ---- beam.cu
+struct BeamArgs {
+  const void* logits;  // [batch * beams][ld]
+  long long ld;
+  int f32;
+  const float* scores;        // [batch][beams]
+  const unsigned char* fin;   // [batch][beams] or null
+  int batch, beams, vocab, n_out, eos;
+  int* parent;
+  int* token;
+  float* out;
+  unsigned char* fin_out;  // or null
+  int splits, slice;       // vocabulary slices per row, elements per slice
+  int vec;                 // rows readable by 16-byte loads
+  float2* cand;            // workspace [batch * beams][splits][n_out]: (logit, index bits), best first
+  float2* stat;            // workspace [batch * beams][splits]: (max, sum exp(x - max))
+};
+constexpr int kBeamMaxOut = 128;
+constexpr int kBeamMaxBeams = 128;
+void beam_split(int batch, int beams, int vocab, int* splits, int* slice);
+cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t st);
+
+struct ReorderTensor {
+  const char* src;
+  char* dst;
+  long long src_stride, dst_stride, seg_stride;
+  long long seg_bytes;
+  int n_seg;
+  int width;  // bytes per column access: 16, 8, 4, 2 or 1
+};
+constexpr int kReorderBatch = 48;  // tensors per launch
+constexpr int kReorderMaxOut = 64;
+struct ReorderArgs {
+  ReorderTensor t[kReorderBatch];
+  long long first[kReorderBatch + 1];  // first block of each tensor, then the total
+  int n;
+  const int* parent;
+  int batch, beams, n_out;
+};
+cudaError_t launch_reorder(ReorderArgs& a, cudaStream_t st);
+
+// ---- runtime.cu
+void set_last_error(const std::string& msg);
+void note_launches(int n);
+
+}  // namespace llmoc

@@ -2197,11 +2197,14 @@ llmoc_status llmoc_ep_p2p_finish(const llmoc_moe_layer* L, llmoc_ep_transport* t
 namespace llmoc {
 // Device a layer lives on (used by the allocation-free entry point in no_alloc.cu).
 int layer_device(const llmoc_moe_layer* L) { return L ? L->device : -1; }
+int layer_hidden(const llmoc_moe_layer* L) { return L ? L->d.hidden : 0; }
 }  // namespace llmoc
 
 namespace llmoc {
 // Sets the text llmoc_last_error() returns on this thread.
 void set_last_error(const std::string& msg) { t_err = msg; }
+// Adds to llmoc_kernel_launch_count() (the operators of ops_runtime.cu).
+void note_launches(int n) { count_launch(n); }
 }  // namespace llmoc
 
 // ------------------------------------------------------ NVLink collectives

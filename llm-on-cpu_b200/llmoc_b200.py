@@ -28,6 +28,8 @@ SCHEME_GPTQ_ASYM = 1
 SCHEME_AWQ_SYM = 2
 ROUTER_SOFTMAX = 0
 ROUTER_SIGMOID_BIAS = 1
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
 
 
 class Int4View(C.Structure):
@@ -58,6 +60,31 @@ class RouteViews(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("ids", C.c_void_p), ("weights", C.c_void_p),
                 ("offsets", C.c_void_p), ("sorted", C.c_void_p), ("inverse", C.c_void_p),
                 ("n_active", C.c_void_p), ("error_flag", C.c_void_p)]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [("hidden", C.c_int32), ("post", C.c_int32), ("pre", C.c_int32), ("weight_dtype", C.c_int32),
+                ("post_weight", C.c_void_p), ("post_bias", C.c_void_p), ("pre_weight", C.c_void_p),
+                ("pre_bias", C.c_void_p), ("weight_offset", C.c_float), ("eps", C.c_float),
+                ("block_scale", C.c_float), ("residual_scale", C.c_float), ("gate_act", C.c_int32)]
+
+
+class NormIO(C.Structure):
+    _fields_ = [("block", C.c_void_p), ("ld_block", C.c_int64), ("residual", C.c_void_p), ("ld_residual", C.c_int64),
+                ("residual_out", C.c_void_p), ("ld_residual_out", C.c_int64), ("norm_out", C.c_void_p),
+                ("ld_norm_out", C.c_int64), ("gate", C.c_void_p), ("gate_row_stride", C.c_int64),
+                ("gate_col_stride", C.c_int64), ("block_dtype", C.c_int32), ("residual_dtype", C.c_int32),
+                ("norm_dtype", C.c_int32), ("gate_dtype", C.c_int32)]
+
+
+class BeamDesc(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("n_out", C.c_int32),
+                ("eos_token", C.c_int32)]
+
+
+class ReorderTensor(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_stride", C.c_int64), ("dst_stride", C.c_int64),
+                ("seg_stride", C.c_int64), ("seg_bytes", C.c_int64), ("n_seg", C.c_int32)]
 
 
 _vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
@@ -141,6 +168,18 @@ _SIGS = {
     "llmoc_ep_p2p_workspace_bytes": (_sz, [_vp, _vp, _i]),
     "llmoc_ep_p2p_send": (_i, [_vp, _vp, _vp, _i, C.c_uint32, _vp, _sz, _vp]),
     "llmoc_ep_p2p_serve": (_i, [_vp, _vp, _i, C.c_uint32, _vp, _sz, _vp]),
+    "llmoc_int4_linear_create": (_i, [C.POINTER(Int4View), _i, _i, _i, C.POINTER(_vp)]),
+    "llmoc_int4_linear_destroy": (None, [_vp]),
+    "llmoc_int4_linear_weight_bytes": (_sz, [_vp]),
+    "llmoc_int4_linear_forward": (_i, [_vp, _vp, C.c_int64, _i, _vp, C.c_int64, _vp, C.c_int64, _i, _vp]),
+    "llmoc_norm_residual": (_i, [C.POINTER(NormDesc), C.POINTER(NormIO), _i, _i, _vp]),
+    "llmoc_moe_block_workspace_bytes": (_sz, [_vp, _i]),
+    "llmoc_moe_forward_block": (_i, [_vp, C.POINTER(NormDesc), C.POINTER(NormDesc), C.POINTER(NormIO), _i, _vp, _sz,
+                                     _vp]),
+    "llmoc_beam_workspace_bytes": (_sz, [C.POINTER(BeamDesc)]),
+    "llmoc_beam_select": (_i, [C.POINTER(BeamDesc), _vp, C.c_int64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i,
+                               _vp]),
+    "llmoc_beam_reorder": (_i, [C.POINTER(ReorderTensor), _i, _vp, _i, _i, _i, _i, _vp]),
     "llmoc_ep_p2p_finish": (_i, [_vp, _vp, _vp, _i, _vp, C.c_uint32, _vp, _sz, _vp]),
 }
 for _name, (_res, _args) in _SIGS.items():
@@ -283,6 +322,17 @@ class MoeLayer:
         check(lib.llmoc_moe_forward_residual(self.handle, ptr(X), T, ptr(R), ptr(Y), ptr(ws), ws_bytes,
                                              stream_ptr(stream)), "llmoc_moe_forward_residual")
 
+    def block_workspace_bytes(self, T: int) -> int:
+        return int(lib.llmoc_moe_block_workspace_bytes(self.handle, T))
+
+    def forward_block(self, before: "ResidualNorm", after: "ResidualNorm", T: int, residual, residual_out, norm_out,
+                      ws, ws_bytes: int, gate=None, stream=None) -> None:
+        """The MoE block on its residual stream: before's pre norm, the layer,
+        then after's post norm, gate, scales, residual add and pre norm."""
+        io = after.io(T, None, residual, residual_out, norm_out, gate)
+        check(lib.llmoc_moe_forward_block(self.handle, C.byref(before.desc), C.byref(after.desc), C.byref(io), T,
+                                          ptr(ws), ws_bytes, stream_ptr(stream)), "llmoc_moe_forward_block")
+
     def route(self, X, T: int, ws, ws_bytes: int, stream=None) -> None:
         check(lib.llmoc_moe_route(self.handle, ptr(X), T, ptr(ws), ws_bytes, stream_ptr(stream)),
               "llmoc_moe_route")
@@ -317,6 +367,228 @@ class MoeLayer:
 def quantize_awq_sym(W, M: int, K: int, gs: int, bf16_scale: bool, q, scales, stream=None) -> None:
     check(lib.llmoc_quantize_awq_sym(ptr(W), M, K, gs, int(bf16_scale), ptr(q), ptr(scales),
                                      stream_ptr(stream)), "llmoc_quantize_awq_sym")
+
+
+# ------------------------------------------- operators around the MoE layer
+#
+# Tensors are torch tensors on the operator's device; row strides are taken
+# from them, and a tensor of another device, type or shape is refused here,
+# before the library sees its address.
+
+_DT = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
+
+
+def _dtype(x, what: str) -> int:
+    d = _DT.get(str(x.dtype))
+    if d is None:
+        raise LlmocError(f"{what}: {x.dtype} is not supported (bfloat16 or float32)")
+    return d
+
+
+def _device(x, device: int, what: str) -> int:
+    """The address of a cuda:`device` tensor."""
+    if x.device.type != "cuda" or x.device.index != device:
+        raise LlmocError(f"{what} is on {x.device}, not on cuda:{device}")
+    return x.data_ptr()
+
+
+def _rows(x, rows: int, cols: int, device: int, what: str):
+    """(address, row stride) of a [>= rows, cols] tensor with adjacent columns."""
+    if x.dim() != 2 or x.shape[0] < rows or x.shape[1] != cols:
+        raise LlmocError(f"{what}: shape {tuple(x.shape)}, not [{rows}, {cols}]")
+    if cols > 1 and x.stride(1) != 1:
+        raise LlmocError(f"{what}: columns are not adjacent in memory")
+    return _device(x, device, what), x.stride(0) if rows > 1 else max(x.stride(0), cols)
+
+
+class Int4Linear:
+    """Dense INT4 weights resident on one device (llmoc_int4_linear_*):
+    Y = X . W^T (+ R) for bf16 rows, asynchronous on a stream."""
+
+    def __init__(self, handle: int, M: int, K: int, device: int):
+        self.handle, self.M, self.K, self.device = handle, M, K, device
+
+    @classmethod
+    def create(cls, views: Sequence[Int4View], device: int = 0, on_device: bool = False) -> "Int4Linear":
+        """From one view, or from several that share their input (stacked rows).
+        Host buffers, or with on_device buffers of that device."""
+        arr = (Int4View * len(views))(*views)
+        h = C.c_void_p()
+        check(lib.llmoc_int4_linear_create(arr, len(views), device, 1 if on_device else 0, C.byref(h)),
+              "llmoc_int4_linear_create")
+        return cls(h.value, sum(v.M for v in views), views[0].K, device)
+
+    def forward(self, X, T: int, Y, R=None, stream=None) -> None:
+        """Y[T, M] (bf16 or fp32) = X[T, K] (bf16) . W^T (+ R[T, M] bf16; R may be Y)."""
+        if self.handle is None:
+            raise LlmocError("llmoc_int4_linear_forward: the weights are closed")
+        if T <= 0:
+            check(OK if T == 0 else 1, "llmoc_int4_linear_forward: negative T")
+            return
+        x, ldx = _rows(X, T, self.K, self.device, "X")
+        y, ldy = _rows(Y, T, self.M, self.device, "Y")
+        r, ldr = _rows(R, T, self.M, self.device, "R") if R is not None else (None, 0)
+        if _dtype(X, "X") != DTYPE_BF16 or (R is not None and _dtype(R, "R") != DTYPE_BF16):
+            raise LlmocError("llmoc_int4_linear_forward: X and R are bfloat16")
+        check(lib.llmoc_int4_linear_forward(self.handle, x, ldx, T, r, ldr, y, ldy, _dtype(Y, "Y"),
+                                            stream_ptr(stream)), "llmoc_int4_linear_forward")
+
+    def weight_bytes(self) -> int:
+        return int(lib.llmoc_int4_linear_weight_bytes(self.handle))
+
+    def close(self) -> None:
+        if self.handle:
+            lib.llmoc_int4_linear_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class ResidualNorm:
+    """The norm after a block, its gate and scale, the residual add and the
+    norm before the next block, in one pass (llmoc_norm_residual)."""
+
+    KINDS = {"none": 0, "rms": 1, "layer": 2}
+    ACTS = {"none": 0, "sigmoid": 1}
+
+    def __init__(self, hidden: int, post: str = "none", post_weight=None, post_bias=None, pre: str = "none",
+                 pre_weight=None, pre_bias=None, weight_offset: float = 0.0, eps: float = 1e-6,
+                 block_scale: float = 1.0, residual_scale: float = 1.0, gate_act: str = "none", device: int = 0):
+        self.hidden, self.device = hidden, device
+        self._keep = [w for w in (post_weight, post_bias, pre_weight, pre_bias) if w is not None]
+        for w in self._keep:
+            if w.dim() != 1 or w.shape[0] != hidden or (hidden > 1 and w.stride(0) != 1):
+                raise LlmocError(f"norm weight: shape {tuple(w.shape)}, not a contiguous [{hidden}]")
+            if w.dtype != self._keep[0].dtype:
+                raise LlmocError("norm weights differ in type")
+
+        def at(w):
+            return None if w is None else _device(w, device, "norm weight")
+
+        self.desc = NormDesc(hidden, self.KINDS[post], self.KINDS[pre],
+                             _dtype(self._keep[0], "norm weight") if self._keep else DTYPE_F32, at(post_weight),
+                             at(post_bias), at(pre_weight), at(pre_bias), weight_offset, eps, block_scale,
+                             residual_scale, self.ACTS[gate_act])
+
+    def io(self, T: int, block, residual, residual_out, norm_out, gate) -> NormIO:
+        H, dev = self.hidden, self.device
+        (b, ldb), (r, ldr), (ro, ldro), (no, ldno) = [
+            (None, 0) if x is None else _rows(x, T, H, dev, what)
+            for x, what in ((block, "block"), (residual, "residual"), (residual_out, "residual_out"),
+                            (norm_out, "norm_out"))]
+        rdt = DTYPE_BF16
+        if residual is not None or residual_out is not None:
+            rdt = _dtype(residual if residual is not None else residual_out, "residual")
+            if residual is not None and residual_out is not None and residual.dtype != residual_out.dtype:
+                raise LlmocError("residual and residual_out differ in type")
+        g, gr, gc, gdt = None, 0, 0, DTYPE_BF16
+        if gate is not None:  # [T, H], [1, H], [T, 1] or [1, 1]
+            if gate.dim() != 2 or (gate.shape[0] != 1 and gate.shape[0] < T) or gate.shape[1] not in (1, H):
+                raise LlmocError(f"gate: shape {tuple(gate.shape)}, not [{T} or 1, {H} or 1]")
+            g, gdt = _device(gate, dev, "gate"), _dtype(gate, "gate")
+            gr = gate.stride(0) if gate.shape[0] > 1 else 0
+            gc = gate.stride(1) if gate.shape[1] > 1 else 0
+        return NormIO(b, ldb, r, ldr, ro, ldro, no, ldno, g, gr, gc, DTYPE_BF16 if block is None else _dtype(block, "block"),
+                      rdt, DTYPE_BF16 if norm_out is None else _dtype(norm_out, "norm_out"), gdt)
+
+    def forward(self, T: int, block, residual, residual_out, norm_out, gate=None, stream=None) -> None:
+        """residual_out = residual_scale * residual + block_scale * act(gate) *
+        post(block), norm_out = pre(that); any operand may be None where the
+        desc needs none."""
+        io = self.io(T, block, residual, residual_out, norm_out, gate)
+        check(lib.llmoc_norm_residual(C.byref(self.desc), C.byref(io), T, self.device, stream_ptr(stream)),
+              "llmoc_norm_residual")
+
+
+class BeamSearch:
+    """Selection over beams and vocabulary (llmoc_beam_select) for one shape."""
+
+    def __init__(self, batch: int, beams: int, vocab: int, n_out: int, eos_token: int = -1, device: int = 0):
+        self.desc = BeamDesc(batch, beams, vocab, n_out, eos_token)
+        self.device = device
+
+    def workspace_bytes(self) -> int:
+        return int(lib.llmoc_beam_workspace_bytes(C.byref(self.desc)))
+
+    def _plain(self, x, shape, dtype: str, what: str):
+        if x is None:
+            return None
+        if tuple(x.shape) != shape or str(x.dtype) != dtype or not x.is_contiguous():
+            raise LlmocError(f"{what}: not a contiguous {dtype} tensor of shape {shape}")
+        return _device(x, self.device, what)
+
+    def select(self, logits, scores, parent, token, out_scores, ws, ws_bytes: int, finished=None, finished_out=None,
+               stream=None) -> None:
+        """logits [batch * beams, vocab] (bf16 or fp32), scores [batch, beams]
+        fp32, finished [batch, beams] uint8 -> parent, token (int32),
+        out_scores (fp32), finished_out (uint8), all [batch, n_out]."""
+        d = self.desc
+        rows, kept = (d.batch, d.beams), (d.batch, d.n_out)
+        x, ld = _rows(logits, d.batch * d.beams, d.vocab, self.device, "logits")
+        args = (self._plain(scores, rows, "torch.float32", "scores"),
+                self._plain(finished, rows, "torch.uint8", "finished"),
+                self._plain(parent, kept, "torch.int32", "parent"), self._plain(token, kept, "torch.int32", "token"),
+                self._plain(out_scores, kept, "torch.float32", "out_scores"),
+                self._plain(finished_out, kept, "torch.uint8", "finished_out"))
+        check(lib.llmoc_beam_select(C.byref(d), x, ld, _dtype(logits, "logits"), *args, ptr(ws), ws_bytes, self.device,
+                                    stream_ptr(stream)), "llmoc_beam_select")
+
+
+class BeamReorder:
+    """The beams' states gathered by parent (llmoc_beam_reorder) for one set of
+    tensors, whose addresses are taken here: src[i] [batch, beams, ...] and
+    dst[i] [batch, n_out, ...], contiguous, or [batch * rows, ...]; dst[i] may
+    be src[i] when n_out = beams.  With `used`, only the first `used` indices
+    of dimension `dim` of a row move (a cache filled up to that length)."""
+
+    def __init__(self, src: Sequence, dst: Sequence, batch: int, beams: int, n_out: int, device: int = 0,
+                 dim: int = 0, used: Optional[int] = None):
+        if len(src) != len(dst):
+            raise LlmocError("BeamReorder: as many destinations as sources")
+        self.batch, self.beams, self.n_out, self.device = batch, beams, n_out, device
+        self._keep = (list(src), list(dst))
+        self.tensors = (ReorderTensor * max(1, len(src)))()
+        self.dim, self.n = dim, len(src)
+        self._row = []
+        for i, (s, d) in enumerate(zip(src, dst)):
+            n = [1, 1]
+            for j, (x, rows) in enumerate(((s, beams), (d, n_out))):
+                if not x.is_contiguous() or x.numel() % max(1, batch * rows):
+                    raise LlmocError(f"BeamReorder: tensor {i} is not a contiguous block of {batch} x {rows} rows")
+                n[j] = x.numel() // max(1, batch * rows)
+            shape = tuple(s.shape[2:]) if s.dim() > 1 and tuple(s.shape[:2]) == (batch, beams) else tuple(s.shape[1:])
+            if n[0] != n[1] or s.dtype != d.dtype:
+                raise LlmocError(f"BeamReorder: rows of tensor {i} differ in size or type")
+            self._row.append((shape, s.element_size(), n[0]))
+            size = n[0] * s.element_size()
+            self.tensors[i] = ReorderTensor(_device(s, device, f"src[{i}]"), _device(d, device, f"dst[{i}]"), size, size,
+                                            0, size, 1)
+        if used is not None:
+            self.set_used(used)
+
+    def set_used(self, used: int) -> None:
+        """Move only the first `used` indices of dimension `dim` of every row from now on."""
+        for i, (shape, es, n) in enumerate(self._row):
+            if self.dim >= len(shape) or not 0 <= used <= shape[self.dim]:
+                raise LlmocError(f"BeamReorder: {used} of dimension {self.dim} of rows {shape}")
+            inner = es
+            for v in shape[self.dim + 1:]:
+                inner *= v
+            whole = inner * shape[self.dim]
+            t = self.tensors[i]
+            t.n_seg, t.seg_stride, t.seg_bytes = max(1, n * es // whole if whole else 1), whole, inner * used
+
+    def run(self, parent, stream=None) -> None:
+        """parent [batch, n_out] int32 on the device (outside [0, beams): that row stays)."""
+        if tuple(parent.shape) != (self.batch, self.n_out) or str(parent.dtype) != "torch.int32" \
+                or not parent.is_contiguous():
+            raise LlmocError(f"parent: not a contiguous int32 tensor of shape {(self.batch, self.n_out)}")
+        check(lib.llmoc_beam_reorder(self.tensors, self.n, _device(parent, self.device, "parent"), self.batch,
+                                     self.beams, self.n_out, self.device, stream_ptr(stream)), "llmoc_beam_reorder")
 
 
 def launch_count() -> int:
