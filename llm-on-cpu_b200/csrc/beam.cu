@@ -49,6 +49,13 @@ __device__ __forceinline__ uint32_t order_code(float x) {
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ unsigned long long order_code64(double x) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(x == 0. ? 0. : x);
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+__device__ __forceinline__ double from_code64(unsigned long long c) {
+  return __longlong_as_double((long long)(c >> 63 ? c & ~(1ull << 63) : ~c));
+}
 // a before b in the order "larger value, then smaller index"
 __device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
 
@@ -211,7 +218,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
   __shared__ int kind[kBeamMaxBeams];     // 0 no candidate, 1 live, 2 finished
   __shared__ double list_v[kMergeList];
   __shared__ long long list_i[kMergeList];  // beam * vocab + token
-  __shared__ double grp[kBeamMaxOut];
+  __shared__ unsigned long long grp[kBeamMaxOut];  // order codes
   __shared__ double red_v[kMergeWarps];
   __shared__ long long red_i[kMergeWarps];
   __shared__ int cnt;
@@ -220,6 +227,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
   grid_dep_wait();
   grid_dep_release();
   if (tid == 0) cnt = 0;
+  if (tid < kBeamMaxOut) grp[tid] = 0;
   for (int w = warp; w < W; w += kMergeWarps) {  // a warp per beam: its slices in lane order
     const int row = b * W + w;
     const float sc = a.scores[row];
@@ -262,24 +270,19 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
       *v = base[w], *id = (long long)w * a.vocab + a.eos;
     }
   };
-  // bound: the smallest of the maxima of at least k groups of threads' heads
-  double m = -INFINITY;
+  // bound: the smallest of the maxima of k groups of list heads, neighbouring
+  // lists (slices of one beam) in different groups
+  const int ng = min(k, lists);
   for (int l = tid; l < lists; l += kMergeThreads) {
     double v;
     long long id;
     entry(l, 0, &v, &id);
-    m = fmax(m, v);
+    atomicMax(&grp[l % ng], order_code64(v));
   }
-  int p = 5;
-  while ((kMergeThreads >> p) < k) --p;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1)
-    if (o < (1 << p)) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const int ng = kMergeThreads >> p;
-  if ((lane & ((1 << p) - 1)) == 0) grp[tid >> p] = m;
   __syncthreads();
-  double bound = grp[0];
-  for (int i = 1; i < ng; ++i) bound = fmin(bound, grp[i]);
+  unsigned long long lowest = grp[0];
+  for (int i = 1; i < ng; ++i) lowest = min(lowest, grp[i]);
+  const double bound = lists < k ? -INFINITY : from_code64(lowest);
   for (int l = tid; l < lists; l += kMergeThreads)
     for (int j = 0; j < k; ++j) {
       double v;

@@ -6,16 +6,36 @@
 // small-batch products of a decode step.  What bounds them is reading the
 // weights once: M * K / 2 bytes.
 //
-// One warp owns RT 16-row tiles of W, a block of NT * 8 tokens and a slice of
-// K.  It streams its weights through a ring of kRing 512-byte chunks held in
-// registers: a chunk (16 rows x 64 k) is one coalesced 16-byte load per lane,
-// reissued for the chunk kRing further on as soon as it is consumed, so every
-// warp keeps kRing * 512 bytes in flight.  A word's eight nibbles become the
-// bf16 A fragments of one mma.m16n8k16 (128 + q by one lop3 per pair, then an
-// exact subtraction of 128 + zp), so products and group sums are exact up to
-// the tensor core's fp32 accumulation; each group's fp32 partial is scaled on
-// the accumulator.  Activations are the B fragments, read by 16-byte loads
-// that hit L1 after their first use on an SM.
+// Weights are packed for this kernel (k_lin_pack): per 16-row tile a stream of
+// blocks of 256 k, each four 512-byte chunks of words (64 k: lane L's 16 bytes
+// at 16 L) followed by the block's scales (and zeros) as fp16 pairs of rows
+// (g, g + 8).  Groups that are other multiples of 32, 64 or 128 repeat their
+// scale, so a block holds 8, 4 or 2 groups of 32, 64 or 128.
+//
+// Work.  A warp owns RT tiles against NT * 8 tokens over a slice of K.  The
+// eight warps of a CTA take 8 / ksw tile groups and split K ksw ways; a cluster
+// of c CTAs splits K c ways more.  With c = ksw = 1 a CTA walks tile groups
+// (persistent) and its warps never meet; otherwise the partial sums meet in
+// (distributed) shared memory and are added in slice order, so no workspace is
+// needed and the bits do not depend on timing.
+//
+// The stream runs through a ring of registers, 4 KB per warp: a chunk is one
+// coalesced 16-byte load per lane, reissued for the place 8 / RT chunks further
+// on as soon as it is consumed, across tile ends.
+//
+// Dequantisation.  A word holds eight nibbles, pair j of them (one per 16-bit
+// half) at bits 3 + 4j: rotated right by 4j and merged into 0x4180 it is the
+// bf16 pair 16 + q, exact, two instructions per pair and no subtraction.  With
+// P = sum (16 + q) x from mma.m16n8k16 (exact products, fp32 sums) and the
+// group's activation sum xs, the group adds s * (P - (16 + zp) * xs), or
+// s * (P - 16 xs) + z * xs.  The offset 16 (the smallest power of two above
+// the nibbles) keeps the cancellation to a factor of about five; 128, which
+// needs no positioned nibbles, would lose five bits.
+//
+// Activations are staged once per CTA and K slab in shared memory in B fragment
+// order (lane (g, t): token g, 8 consecutive k from 8 t), one conflict-free
+// 16-byte load per 32 k and 8 tokens, with the group sums beside them.  One
+// token is stored once and read as all eight columns.
 #include <algorithm>
 #include <string>
 
@@ -27,23 +47,25 @@ namespace {
 
 constexpr int kLinWarps = 8;
 constexpr int kLinThreads = kLinWarps * 32;
+constexpr uint32_t kOffset = 16;  // A elements are kOffset + q
 
-__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
+__device__ __forceinline__ uint4 ld_stream(const char* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint32_t nib_pair(uint32_t w) {  // (128 + q_lo, 128 + q_hi) as bf16
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(0x000F000Fu), "r"(0x43004300u));
-  return d;
+__device__ __forceinline__ uint32_t ld_pair(const char* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
 }
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r =
-      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ float2 pair_f32(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ uint32_t nib_pair(uint32_t w) {  // (16 + q_lo, 16 + q_hi) as bf16
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(0x00780078u), "r"(0x41804180u));
+  return d;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -51,169 +73,156 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Eight consecutive activations of one token as four bf16 pairs.
-__device__ __forceinline__ uint4 load_x(const __nv_bfloat16* p, bool ok, int vec) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (ok) {
-    if (vec) {
-      v = __ldg(reinterpret_cast<const uint4*>(p));
-    } else {
-      const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
-      v.x = __ldg(u) | ((uint32_t)__ldg(u + 1) << 16);
-      v.y = __ldg(u + 2) | ((uint32_t)__ldg(u + 3) << 16);
-      v.z = __ldg(u + 4) | ((uint32_t)__ldg(u + 5) << 16);
-      v.w = __ldg(u + 6) | ((uint32_t)__ldg(u + 7) << 16);
-    }
-  }
+// Every CTA of the cluster arrives and waits; shared-memory writes before it
+// are visible to the cluster's CTAs after it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// *p of the cluster's CTA `rank` (c = 1: of this CTA)
+__device__ __forceinline__ float ld_cluster(const float* p, int rank, int c) {
+  if (c == 1) return *p;
+  uint32_t at;
+  float v;
+  const uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
 }
 
-// GSB: 32-wide blocks per scale group: 1, 2 or 4, or 0 for any other multiple
-// (then each block is scaled on its own).
-template <int GSB, bool AWQ, int NT, int RT>
-__global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a) {
-  constexpr int kRing = 8 / RT;
-  constexpr int kGpc = GSB == 2 || GSB == 4 ? 1 : 2;  // scale pairs fetched per 64-wide chunk
-  constexpr int kRows = RT * 16, kCols = NT * 8, kColLd = kRows + 4;
-  __shared__ float red[kLinWarps][kCols * kColLd];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tb = blockIdx.x % a.ntb;
-  const int ks = a.ks, upc = kLinWarps / ks;
-  const int u0 = (blockIdx.x / a.ntb) * upc;            // first unit of the CTA
-  const int unit = u0 + warp / ks, sl = warp % ks;
-  const int nu = (a.mt + RT - 1) / RT;
-  int c0 = 0, c1 = 0;
-  if (unit < nu) {  // slices of whole chunk pairs (a group of 128 never straddles two)
-    const int pairs = (a.Kc + 1) >> 1;
-    c0 = min(a.Kc, 2 * (int)((long long)pairs * sl / ks));
-    c1 = min(a.Kc, 2 * (int)((long long)pairs * (sl + 1) / ks));
-  }
-  int tile[RT];
-  const uint4* qp[RT];
-  const __half2* sp[RT];
-  const __half2* zp[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {  // a tile past the end repeats the last one; its rows are not stored
-    tile[r] = min(unit * RT + r, a.mt - 1);
-    qp[r] = a.q + (size_t)tile[r] * a.Kc * 32 + piece_slot(lane);
-    sp[r] = a.s + (size_t)tile[r] * a.ng * 8 + g;
-    zp[r] = AWQ ? nullptr : a.z + (size_t)tile[r] * a.ng * 8 + g;
-  }
-  // scale group of block kb of chunk c
-  const int gsb = a.gs >> 5;
-  auto grp = [&](int c, int kb) { return GSB == 4 ? c >> 1 : GSB == 2 ? c : GSB == 1 ? 2 * c + kb : (2 * c + kb) / gsb; };
-  auto ld_s = [&](const __half2* p, int c, int kb) { return __ldg(p + (size_t)min(grp(c, kb), a.ng - 1) * 8); };
+struct LinPlan {
+  int lk;     // log2 of ksw, the warps of a CTA that split K
+  int lc;     // log2 of c, the CTAs of a cluster that split K
+  int units;  // tile groups (8 / ksw warps x RT tiles)
+  int bps;    // blocks of 256 k per staged slab
+  int nslab;  // slabs of a CTA's share of K
+};
 
-  uint4 qw[kRing][RT];
-  __half2 sw[kRing][RT][kGpc], zw[kRing][RT][kGpc];
-  auto fetch = [&](int i, int c) {
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      qw[i][r] = ld_stream(qp[r] + (size_t)c * 32);
-#pragma unroll
-      for (int kb = 0; kb < kGpc; ++kb) {
-        sw[i][r][kb] = ld_s(sp[r], c, kb);
-        if (!AWQ) zw[i][r][kb] = ld_s(zp[r], c, kb);
-      }
-    }
+// FL: 32-wide blocks per scale group (1, 2, 4); TP: token rows staged (1, or
+// NT * 8).
+template <int FL, bool AWQ, int NT, int RT, int TP>
+__global__ void __launch_bounds__(kLinThreads, NT * RT >= 6 ? 1 : 2) k_linear(const LinArgs a, const LinPlan p) {
+  constexpr int kBB = lin_block_bytes(FL, !AWQ);
+  constexpr int GB = 2 / RT;                    // blocks in flight per tile
+  constexpr int kGrp = 8 / FL;                  // scale groups per block
+  constexpr int kRows = RT * 16, kCols = NT * 8, kColLd = kRows + 4;
+  constexpr int kXW = TP * 4;                   // 16-byte pieces per 32 k
+  extern __shared__ __align__(16) uint4 sx[];   // [slab's 32-blocks][kXW]: B fragments
+  float* xs = reinterpret_cast<float*>(sx + (size_t)p.bps * 8 * kXW);  // [slab's groups][TP]: activation sums
+  float* red = xs + (size_t)p.bps * kGrp * TP;                         // [warp][col][row]: partial sums
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int c = 1 << p.lc, ksw = 1 << p.lk, lr = 3 - p.lk;  // lr: log2 of the CTA's tile groups
+  const int rank = blockIdx.x & (c - 1), ncl = gridDim.x >> p.lc;
+  const int tok0 = blockIdx.y * kCols;
+  const int wt = warp & ((1 << lr) - 1), wk = warp >> lr;
+  const int p0 = a.nb * rank >> p.lc, p1 = a.nb * (rank + 1) >> p.lc;  // nb < 2^23
+  const int nslab = p.nslab;
+
+  // segment (unit, slab) of this warp: its first block within the slab, its
+  // blocks and their address
+  struct Seg {
+    const char* q;
+    int b0, nb;
   };
+  const size_t tile_bytes = (size_t)a.nb * kBB;
+  auto seg_of = [&](int unit, int slab) {
+    Seg s;
+    const int s0 = p0 + slab * p.bps, n = max(0, min(p1, s0 + p.bps) - s0);
+    const int tile = ((unit << lr) + wt) * RT;
+    s.b0 = n * wk >> p.lk;
+    s.nb = tile < a.mt && unit < p.units ? (n * (wk + 1) >> p.lk) - s.b0 : 0;
+    s.q = a.q + (size_t)min(tile, a.mt - 1) * tile_bytes + (size_t)(s0 + s.b0) * kBB;
+    return s;
+  };
+  uint4 qw[GB][4][RT];
+  uint32_t sw[GB][kGrp][RT], zw[GB][kGrp][RT];
+  // a tile past the end reads the last one again; its rows are not stored
+  auto tile_off = [&](int r, int unit) { return r && ((unit << lr) + wt) * RT + r < a.mt ? tile_bytes : 0; };
+  const int lq = lane * 16, ls = 2048 + g * 4;
+
+  int unit = blockIdx.x >> p.lc, slab = 0;
+  Seg cur = seg_of(unit, 0);
 #pragma unroll
-  for (int i = 0; i < kRing; ++i)
-    if (c0 + i < c1) fetch(i, c0 + i);  // weights do not depend on the previous kernel
+  for (int j = 0; j < GB; ++j)  // the weights do not depend on the previous kernel
+    if (j < cur.nb)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const char* q = cur.q + tile_off(r, unit) + j * kBB;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qw[j][i][r] = ld_stream(q + lq + i * 512);
+#pragma unroll
+        for (int i = 0; i < kGrp; ++i) {
+          sw[j][i][r] = ld_pair(q + ls + i * 32);
+          if (!AWQ) zw[j][i][r] = ld_pair(q + ls + (kGrp + i) * 32);
+        }
+      }
   grid_dep_wait();
   grid_dep_release();
 
-  float acc[RT][NT][4], part[RT][NT][4], xs[NT][4];
+  float acc[RT][NT][4], part[RT][NT][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xs[n][i] = 0.f;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) acc[r][n][i] = part[r][n][i] = 0.f;
-    }
-  }
-  const uint32_t zoff = AWQ ? (0x4300u + (uint32_t)a.zp) * 0x10001u : 0x43004300u;  // 128 + zp, exact below 256
-  const int tok0 = tb * kCols + g;
-  const __nv_bfloat16* xp = a.X + (long long)tok0 * a.ldx + 8 * t;
+      for (int i = 0; i < 4; ++i) acc[r][n][i] = part[r][n][i] = 0.f;
+  const float zoff = AWQ ? -(float)(kOffset + a.zp) : -(float)kOffset;
+  const uint4* xl = sx + (TP == 1 ? t : lane);
+  const float* xsl = xs + (TP == 1 ? 0 : 2 * t);
 
-  auto flush = [&](const __half2 (&s)[RT], const __half2 (&z)[RT]) {
+  auto flush = [&](const float* xg, const uint32_t (&s)[RT], const uint32_t (&z)[RT]) {  // xg: the group's sums
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const float2 sf = __half22float2(s[r]);
-      float2 zf = make_float2(0.f, 0.f);
-      if (!AWQ) zf = __half22float2(z[r]);
+    for (int n = 0; n < NT; ++n) {
+      float2 x;
+      if (TP == 1)
+        x.x = x.y = *xg;
+      else
+        x = *reinterpret_cast<const float2*>(xg + n * 8);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        acc[r][n][0] = fmaf(sf.x, part[r][n][0], acc[r][n][0]);
-        acc[r][n][1] = fmaf(sf.x, part[r][n][1], acc[r][n][1]);
-        acc[r][n][2] = fmaf(sf.y, part[r][n][2], acc[r][n][2]);
-        acc[r][n][3] = fmaf(sf.y, part[r][n][3], acc[r][n][3]);
+      for (int r = 0; r < RT; ++r) {
+        const float2 sf = pair_f32(s[r]);
+        float (&o)[4] = acc[r][n];
+        float (&q)[4] = part[r][n];
         if (!AWQ) {
-          acc[r][n][0] = fmaf(zf.x, xs[n][0], acc[r][n][0]);
-          acc[r][n][1] = fmaf(zf.x, xs[n][1], acc[r][n][1]);
-          acc[r][n][2] = fmaf(zf.y, xs[n][0], acc[r][n][2]);
-          acc[r][n][3] = fmaf(zf.y, xs[n][1], acc[r][n][3]);
+          const float2 zf = pair_f32(z[r]);
+          o[0] = fmaf(zf.x, x.x, o[0]), o[1] = fmaf(zf.x, x.y, o[1]);
+          o[2] = fmaf(zf.y, x.x, o[2]), o[3] = fmaf(zf.y, x.y, o[3]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[r][n][i] = 0.f;
+        o[0] = fmaf(sf.x, fmaf(zoff, x.x, q[0]), o[0]), o[1] = fmaf(sf.x, fmaf(zoff, x.y, q[1]), o[1]);
+        o[2] = fmaf(sf.y, fmaf(zoff, x.x, q[2]), o[2]), o[3] = fmaf(sf.y, fmaf(zoff, x.y, q[3]), o[3]);
+        q[0] = q[1] = q[2] = q[3] = 0.f;
       }
-    }
-    if (!AWQ) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xs[n][i] = 0.f;
     }
   };
 
-  for (int cb = c0; cb < c1; cb += kRing) {
-#pragma unroll
-    for (int i = 0; i < kRing; ++i) {
-      const int c = cb + i;
-      if (c >= c1) break;  // uniform over the warp
-      uint32_t w[RT][4];
-      __half2 s[kGpc][RT], z[kGpc][RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        w[r][0] = qw[i][r].x, w[r][1] = qw[i][r].y, w[r][2] = qw[i][r].z, w[r][3] = qw[i][r].w;
-#pragma unroll
-        for (int kb = 0; kb < kGpc; ++kb) {
-          s[kb][r] = sw[i][r][kb];
-          if (!AWQ) z[kb][r] = zw[i][r][kb];
+  // one slab of activations: rows tok0 .., blocks [s0, s0 + bps); zeros past T and K
+  auto stage = [&](int s0, int s1) {
+    const int np = (s1 - s0) * 32;  // 16-byte pieces of a row; a warp's 32 lie in one row
+    int row = 0;
+    for (int pc = threadIdx.x;; pc += kLinThreads) {
+      while (pc >= np && row < TP) pc -= np, ++row;
+      if (row >= TP) break;
+      const int tok = tok0 + row, k = s0 * 256 + pc * 8;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (tok < a.T && k < a.K) {
+        const __nv_bfloat16* src = a.X + (long long)tok * a.ldx + k;
+        if (a.x_vec) {
+          v = *reinterpret_cast<const uint4*>(src);
+        } else {
+          const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+          v.x = u[0] | ((uint32_t)u[1] << 16), v.y = u[2] | ((uint32_t)u[3] << 16);
+          v.z = u[4] | ((uint32_t)u[5] << 16), v.w = u[6] | ((uint32_t)u[7] << 16);
         }
       }
-      if (c + kRing < c1) fetch(i, c + kRing);
+      const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+      float s = 0.f;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const int k = c * 64 + kb * 32;
-        uint4 x[NT];
+      for (int i = 0; i < 4; ++i) s += __uint_as_float(wd[i] << 16) + __uint_as_float(wd[i] & 0xFFFF0000u);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          x[n] = load_x(xp + (long long)n * 8 * a.ldx + k, tok0 + n * 8 < a.T && k < a.K, a.x_vec);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          if (!AWQ) {
-            const uint32_t ones[4] = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(xs[n], ones, kt ? x[n].z : x[n].x, kt ? x[n].w : x[n].y);
-          }
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const uint32_t v = w[r][kb * 2 + kt];
-            uint32_t f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = sub2(nib_pair(v >> (4 * j)), zoff);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(part[r][n], f, kt ? x[n].z : x[n].x, kt ? x[n].w : x[n].y);
-          }
-        }
-        if (kGpc == 2) flush(s[kb], z[kb]);
-      }
-      if (GSB == 2 || (GSB == 4 && ((c & 1) || c + 1 == c1))) flush(s[0], z[0]);
+      for (int o = 1; o < 4 * FL; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      sx[(size_t)(pc >> 2) * kXW + (row >> 3) * 32 + (row & 7) * 4 + (pc & 3)] = v;
+      if ((pc & (4 * FL - 1)) == 0) xs[(pc / (4 * FL)) * TP + row] = s;
     }
-  }
+  };
 
   auto store = [&](int row, int tok, float v) {
     if (row >= a.M || tok >= a.T) return;
@@ -223,65 +232,243 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a) {
     else
       reinterpret_cast<__nv_bfloat16*>(a.Y)[(long long)tok * a.ldy + row] = __float2bfloat16_rn(v);
   };
-  // partial sums of the K slices meet in shared memory and are added in slice order
+
+  bool staged = false;
+  while (unit < p.units) {  // the same for all CTAs of a cluster
+    if (!staged || nslab > 1) {
+      const int s0 = p0 + slab * p.bps;
+      if (staged) __syncthreads();  // the slab before is read no more
+      stage(s0, min(p1, s0 + p.bps));
+      __syncthreads();
+      staged = true;
+    }
+    const int nslab1 = slab + 1 < nslab ? slab + 1 : 0, nunit = nslab1 ? unit : unit + ncl;
+    const Seg nxt = seg_of(nunit, nslab1);
+    const uint4* xb = xl + (size_t)cur.b0 * 8 * kXW;
+    const float* xg = xsl + cur.b0 * kGrp * TP;
+    for (int b = 0; b < cur.nb || b == 0; b += GB) {
+      const bool last = b + GB >= cur.nb;
+      const char* src = last ? nxt.q : cur.q + (size_t)(b + GB) * kBB;
+      const int left = last ? nxt.nb : cur.nb - b - GB;  // blocks to fetch from src
+      const size_t off = RT > 1 ? tile_off(1, last ? nunit : unit) : 0;
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+      for (int j = 0; j < GB; ++j) {
+        const bool more = j < left;
+        const char* sq = src + j * kBB;
+        if (b + j < cur.nb) {  // uniform over the warp
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[RT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[warp][(n * 8 + 2 * t + (i & 1)) * kColLd + r * 16 + g + (i >> 1) * 8] = acc[r][n][i];
-  __syncthreads();
-  const int rows_cta = upc * kRows;
-  for (int e = threadIdx.x; e < rows_cta * kCols; e += kLinThreads) {
-    const int row = e % rows_cta, col = e / rows_cta, w0 = row / kRows * ks;
-    float v = 0.f;
-    for (int s = 0; s < ks; ++s) v += red[w0 + s][col * kColLd + row % kRows];
-    store(u0 * kRows + row, tb * kCols + col, v);
+            for (int r = 0; r < RT; ++r) {
+              w[r][0] = qw[j][i][r].x, w[r][1] = qw[j][i][r].y, w[r][2] = qw[j][i][r].z, w[r][3] = qw[j][i][r].w;
+              if (more) qw[j][i][r] = ld_stream(sq + (r ? off : 0) + lq + i * 512);
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              uint4 x[NT];
+#pragma unroll
+              for (int n = 0; n < NT; ++n) x[n] = xb[(2 * i + kb) * kXW + n * 32];
+#pragma unroll
+              for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                  const uint32_t v = w[r][kb * 2 + kt];
+                  uint32_t f[4];
+#pragma unroll
+                  for (int h = 0; h < 4; ++h) f[h] = nib_pair(__funnelshift_r(v, v, 4 * h));
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) mma16816(part[r][n], f, kt ? x[n].z : x[n].x, kt ? x[n].w : x[n].y);
+                }
+              if ((2 * i + kb) % FL == FL - 1) {
+                const int gi = (2 * i + kb) / FL;
+                flush(xg + gi * TP, sw[j][gi], zw[j][gi]);
+                if (more)
+#pragma unroll
+                  for (int r = 0; r < RT; ++r) {
+                    sw[j][gi][r] = ld_pair(sq + (r ? off : 0) + ls + gi * 32);
+                    if (!AWQ) zw[j][gi][r] = ld_pair(sq + (r ? off : 0) + ls + (kGrp + gi) * 32);
+                  }
+              }
+            }
+          }
+          xb += 8 * kXW;
+          xg += kGrp * TP;
+        } else if (more) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qw[j][i][r] = ld_stream(sq + (r ? off : 0) + lq + i * 512);
+#pragma unroll
+            for (int i = 0; i < kGrp; ++i) {
+              sw[j][i][r] = ld_pair(sq + (r ? off : 0) + ls + i * 32);
+              if (!AWQ) zw[j][i][r] = ld_pair(sq + (r ? off : 0) + ls + (kGrp + i) * 32);
+            }
+          }
+        }
+      }
+    }
+    cur = nxt;
+    if (nslab1 == 0) {  // the unit's last slab
+      if (p.lk == 0 && p.lc == 0) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              store((((unit << lr) + wt) * RT + r) * 16 + g + (i >> 1) * 8, tok0 + n * 8 + 2 * t + (i & 1), acc[r][n][i]);
+      } else {
+        // partial sums of the K slices, added in slice order (rank, then warp);
+        // such a grid has a cluster per unit, so the buffer is written once
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              red[(warp * kCols + n * 8 + 2 * t + (i & 1)) * kColLd + r * 16 + g + (i >> 1) * 8] = acc[r][n][i];
+        if (c > 1)
+          cluster_sync();
+        else
+          __syncthreads();
+        constexpr int kLrow = RT == 1 ? 4 : 5;  // log2 of kRows
+        const int lrows = lr + kLrow, step = kLinThreads << p.lc;
+        const int cols = min(kCols, a.T - tok0);
+        for (int e = threadIdx.x + rank * kLinThreads; e < cols << lrows; e += step) {
+          const int row = e & ((1 << lrows) - 1), col = e >> lrows, w0 = row >> kLrow;
+          const float* at = red + (w0 * kCols + col) * kColLd + (row & (kRows - 1));
+          float v = 0.f;
+          for (int q = 0; q < c; ++q)
+            for (int s = 0; s < ksw; ++s) v += ld_cluster(at + (s << lr) * kCols * kColLd, q, c);
+          store((unit << lrows) + row, tok0 + col, v);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
+    }
+    unit = nunit;
+    slab = nslab1;
+  }
+  if (c > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
+}
+
+constexpr int kLinSmemMax = 100 * 1024;  // two CTAs per SM
+constexpr long long kLinBusy = 148 * 12;
+
+template <int FL, bool AWQ, int NT, int RT, int TP>
+cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
+  LinPlan p{};
+  const int ntb = (a.T + NT * 8 - 1) / (NT * 8);
+  const int tg = (a.mt + RT - 1) / RT;
+  // Split K while the machine has fewer than 16 busy warps per SM: inside the
+  // CTA as long as its activations stay below half of its weights, then over a
+  // cluster, then inside the CTA at any price.
+  int ksw = 1, c = 1;
+  auto busy = [&]() { return (long long)tg * ntb * ksw * c >= kLinBusy || a.nb < 2 * ksw * c; };
+  while (!busy() && ksw < kLinWarps && TP * ksw * 2 <= 16 * RT) ksw *= 2, ++p.lk;
+  while (!busy() && c < 8) c *= 2, ++p.lc;
+  while (!busy() && ksw < kLinWarps) ksw *= 2, ++p.lk;
+  const int rbt = kLinWarps / ksw;
+  p.units = (tg + rbt - 1) / rbt;
+  const bool split = ksw > 1 || c > 1;
+  const int red = split ? kLinWarps * NT * 8 * (RT * 16 + 4) * 4 : 0;
+  const int per_block = TP * 4 * 8 * 16 + 8 / FL * TP * 4;
+  const int share = (a.nb + c - 1) / c;
+  p.bps = std::max(1, std::min(share, (kLinSmemMax - red) / per_block));
+  p.nslab = (share + p.bps - 1) / p.bps;
+  const int smem = p.bps * per_block + red;
+  const auto kernel = k_linear<FL, AWQ, NT, RT, TP>;
+  static bool attr[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmemMax);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr[dev] = true;
+  }
+  const long long gx = (split ? p.units : std::min(p.units, std::max(1, 148 * 2 / ntb))) * (long long)c;
+  if (gx > 0x7FFFFFFFll || ntb > 65535) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)gx, (unsigned)ntb);
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)c;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = c > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a, p);
+}
+
+template <int FL, bool AWQ>
+cudaError_t launch_fl(const LinArgs& a, cudaStream_t st) {
+  // token blocks of up to 32, as even as multiples of 8 allow
+  const int n8 = (a.T + 7) / 8, ntb = (n8 + 3) / 4;
+  switch ((n8 + ntb - 1) / ntb) {
+    case 1: return a.T == 1 ? launch_shape<FL, AWQ, 1, 1, 1>(a, st) : launch_shape<FL, AWQ, 1, 1, 8>(a, st);
+    case 2: return launch_shape<FL, AWQ, 2, 2, 16>(a, st);
+    case 3: return launch_shape<FL, AWQ, 3, 2, 24>(a, st);
+    default: return launch_shape<FL, AWQ, 4, 2, 32>(a, st);
   }
 }
 
-template <int GSB, bool AWQ>
-cudaError_t launch_gs(LinArgs a, cudaStream_t st) {
-  const int nt = a.T <= 8 ? 1 : a.T <= 16 ? 2 : 4;
-  const int rt = nt == 1 ? 1 : 2;
-  a.ntb = (a.T + nt * 8 - 1) / (nt * 8);
-  const int units = (a.mt + rt - 1) / rt;
-  // K split: as few warps per tile as give the machine 16 warps per SM
-  int ks = 1;
-  while (ks < kLinWarps && (long long)units * a.ntb * ks < 148 * 16 && a.Kc >= 4 * ks) ks *= 2;
-  a.ks = ks;
-  const int upc = kLinWarps / ks;
-  const dim3 grid((unsigned)((long long)((units + upc - 1) / upc) * a.ntb));
-  if (nt == 1) return launch_pdl(k_linear<GSB, AWQ, 1, 1>, grid, dim3(kLinThreads), 0, st, a);
-  if (nt == 2) return launch_pdl(k_linear<GSB, AWQ, 2, 2>, grid, dim3(kLinThreads), 0, st, a);
-  return launch_pdl(k_linear<GSB, AWQ, 4, 2>, grid, dim3(kLinThreads), 0, st, a);
-}
-
-__global__ void k_pair_rows(uint16_t* s, size_t n) {
-  const size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  uint16_t v[16];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) v[r] = s[i * 16 + r];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) s[i * 16 + (r & 7) * 2 + (r >> 3)] = v[r];
+// One 32-bit word of the stream per thread: words of a block (rows past M and
+// columns past K are 0, which zero activations meet), then its scale pairs.
+__global__ void k_lin_pack(const LinPack a) {
+  const int bw = lin_block_bytes(a.fl, a.gptq) / 4, grp = 8 / a.fl;
+  const size_t n = (size_t)((a.M + 15) / 16) * a.nb * bw;
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+    const int in = (int)(i % bw);
+    const size_t tb = i / bw;
+    const int b = (int)(tb % a.nb);
+    const long long r0 = (long long)(tb / a.nb) * 16;
+    uint32_t v = 0;
+    if (in < 512) {
+      const int wd = in & 3, lane = (in >> 2) & 31, g = lane >> 2, t = lane & 3;
+      const int k = b * 256 + (in >> 7) * 64 + (wd >> 1) * 32 + t * 8 + (wd & 1) * 4;
+      for (int e = 0; e < 4; ++e)
+        for (int h = 0; h < 2; ++h) {
+          const long long row = r0 + g + 8 * h;
+          if (row >= a.M || k + e >= a.K) continue;
+          const uint32_t byte = a.q[(size_t)row * (a.K / 2) + ((k + e) >> 1)];
+          const uint32_t nib = e & 1 ? byte >> 4 : byte & 15;
+          v |= nib << (4 * ((e & 1) * 4 + (e >> 1) * 2 + h));
+        }
+      v = __funnelshift_l(v, v, 3);
+    } else {
+      const int s = in - 512, z = s / (8 * grp), gi = s / 8 % grp, g = s % 8;
+      const int k = b * 256 + gi * a.fl * 32;
+      const uint16_t* src = z ? a.z : a.s;
+      for (int h = 0; h < 2; ++h) {
+        const long long row = r0 + g + 8 * h;
+        if (row < a.M && k < a.K && src) v |= (uint32_t)src[(size_t)row * a.ng + k / a.gs] << (16 * h);
+      }
+    }
+    a.out[i] = v;
+  }
 }
 
 }  // namespace
 
-cudaError_t launch_pair_rows(uint16_t* s, size_t n, cudaStream_t st) {
-  if (n == 0) return cudaSuccess;
-  k_pair_rows<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(s, n);
+cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st) {
+  k_lin_pack<<<148 * 8, 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 
-cudaError_t launch_linear(const LinArgs& a, bool awq, cudaStream_t st) {
-  switch (a.gs) {
-    case 32: return awq ? launch_gs<1, true>(a, st) : launch_gs<1, false>(a, st);
-    case 64: return awq ? launch_gs<2, true>(a, st) : launch_gs<2, false>(a, st);
-    case 128: return awq ? launch_gs<4, true>(a, st) : launch_gs<4, false>(a, st);
-    default: return awq ? launch_gs<0, true>(a, st) : launch_gs<0, false>(a, st);
+cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st) {
+  switch (fl) {
+    case 1: return awq ? launch_fl<1, true>(a, st) : launch_fl<1, false>(a, st);
+    case 2: return awq ? launch_fl<2, true>(a, st) : launch_fl<2, false>(a, st);
+    default: return awq ? launch_fl<4, true>(a, st) : launch_fl<4, false>(a, st);
   }
 }
 

@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads) k_n
     }
   };
 
+  auto act = [&](float v) { return a.gate_sigmoid ? 1.f / (1.f + expf(-v)) : v; };
   float r[N];
   if (a.res)
     load(a.res, row * a.ld_res, a.res_f32, r, 0.f);
@@ -200,15 +201,15 @@ __global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads) k_n
     if (a.gate) {
       float gt[N];
       const long long off = row * a.gate_row;
-      if (a.gate_col == 0) {
-        const float one = load1(a.gate, off, a.gate_f32);
+      if (a.gate_col == 0) {  // one value a row
+        const float one = act(load1(a.gate, off, a.gate_f32));
 #pragma unroll
-        for (int j = 0; j < N; ++j) gt[j] = one;
+        for (int j = 0; j < N; ++j) x[j] *= one;
       } else {
         load(a.gate, off, a.gate_f32, gt, 0.f);
-      }
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] *= a.gate_sigmoid ? 1.f / (1.f + expf(-gt[j])) : gt[j];
+        for (int j = 0; j < N; ++j) x[j] *= act(gt[j]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) r[j] = fmaf(a.block_scale, x[j], a.res_scale * r[j]);

@@ -11,12 +11,14 @@
 namespace llmoc {
 
 // ---- linear.cu
+// Bytes of a 256-wide block of a tile's stream: 2048 of words, then 32 for each
+// group of fl * 32 (twice with zeros).
+__host__ __device__ constexpr int lin_block_bytes(int fl, bool gptq) { return 2048 + 8 / fl * 32 * (gptq ? 2 : 1); }
 struct LinArgs {
-  const uint4* q;   // fragment order (common.cuh)
-  const __half2* s; // [Mt][ng][8]: the scales of rows g and g + 8 of a tile side by side
-  const __half2* z; // GPTQ zeros, same layout, or null
-  int M, K, Kc, ng, gs;
-  int mt;           // 16-row tiles
+  const char* q;  // the packed stream
+  int M, K;
+  int nb;         // blocks of 256 k per tile
+  int mt;         // 16-row tiles
   int zp;
   const __nv_bfloat16* X;
   long long ldx;
@@ -26,13 +28,17 @@ struct LinArgs {
   void* Y;
   long long ldy;
   int y_f32;
-  int x_vec;        // X rows readable by 16-byte loads
-  int ks;           // warps of a CTA that split K
-  int ntb;          // token blocks
+  int x_vec;  // X rows readable by 16-byte loads
 };
-// [n][16] fp16 (rows of a tile) -> the same 16 values as pairs (g, g + 8), in place
-cudaError_t launch_pair_rows(uint16_t* s, size_t n, cudaStream_t st);
-cudaError_t launch_linear(const LinArgs& a, bool awq, cudaStream_t st);
+struct LinPack {
+  const uint8_t* q;   // QLWC [M][K / 2]
+  const uint16_t* s;  // [M][ng] fp16
+  const uint16_t* z;  // or null
+  int M, K, gs, ng, nb, fl, gptq;
+  uint32_t* out;
+};
+cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st);
+cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st);
 
 // ---- norm.cu
 struct NormArgs {

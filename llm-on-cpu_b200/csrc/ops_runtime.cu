@@ -24,12 +24,10 @@ int layer_hidden(const llmoc_moe_layer* L);
 
 struct llmoc_int4_linear {
   int device = 0;
-  int M = 0, K = 0, Kc = 0, gs = 0, ng = 0, mt = 0, zp = 7;
+  int M = 0, K = 0, nb = 0, mt = 0, zp = 7;
+  int fl = 4;  // 32-wide blocks per packed scale group
   bool awq = true;
   char* arena = nullptr;
-  const uint4* q = nullptr;
-  const __half2* s = nullptr;
-  const __half2* z = nullptr;
   size_t weight_bytes = 0;
 };
 
@@ -148,14 +146,14 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
   L->device = device;
   L->M = (int)M;
   L->K = K;
-  L->Kc = (K + 63) / 64;
-  L->gs = gs;
-  L->ng = (K + gs - 1) / gs;
+  L->nb = (K + 255) / 256;
   L->mt = (int)((M + 15) / 16);
   L->zp = zp;
+  L->fl = gs % 128 == 0 ? 4 : gs % 64 == 0 ? 2 : 1;
   L->awq = awq;
-  const size_t qb = (size_t)L->mt * L->Kc * 512, sb = (size_t)L->mt * L->ng * 32;
-  L->weight_bytes = qb + sb * (awq ? 1 : 2);
+  const int ng = (K + gs - 1) / gs;
+  const size_t tile_bytes = (size_t)L->nb * lin_block_bytes(L->fl, !awq);
+  L->weight_bytes = (size_t)L->mt * tile_bytes;
   cudaStream_t st = nullptr;
   void* staging = nullptr;
   llmoc_status rc = LLMOC_OK;
@@ -167,24 +165,19 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
   };
   do {
     if (!cuda(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking), LLMOC_ERR_CUDA)) break;
-    if (!cuda(cudaMalloc((void**)&L->arena, up256(qb) + up256(sb) * (awq ? 1 : 2)), LLMOC_ERR_NO_MEMORY)) break;
-    char* qo = L->arena;
-    char* so = qo + up256(qb);
-    char* zo = awq ? nullptr : so + up256(sb);
-    L->q = (const uint4*)qo;
-    L->s = (const __half2*)so;
-    L->z = (const __half2*)zo;
+    if (!cuda(cudaMalloc((void**)&L->arena, L->weight_bytes), LLMOC_ERR_NO_MEMORY)) break;
+    char* at = L->arena;
     size_t need = 0;  // staging of the largest host view
     for (int i = 0; i < n_views && !on_device; ++i) {
-      const size_t n = up256((size_t)views[i].M * (K / 2)) + 2 * up256((size_t)views[i].M * L->ng * 2);
+      const size_t n = up256((size_t)views[i].M * (K / 2)) + 2 * up256((size_t)views[i].M * ng * 2);
       need = n > need ? n : need;
     }
     if (need && !cuda(cudaMalloc(&staging, need), LLMOC_ERR_NO_MEMORY)) break;
     for (int i = 0; i < n_views && rc == LLMOC_OK; ++i) {
       const llmoc_int4_view& v = views[i];
-      const size_t qsrc = (size_t)v.M * (K / 2), ssrc = (size_t)v.M * L->ng * 2;
+      const size_t qsrc = (size_t)v.M * (K / 2), ssrc = (size_t)v.M * ng * 2;
       const uint16_t* vz = awq ? nullptr : v.zeros;
-      RepackArgs ra{};
+      LinPack ra{};
       ra.q = v.qweight;
       ra.s = v.scales;
       ra.z = vz;
@@ -204,23 +197,16 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
       ra.M = v.M;
       ra.K = K;
       ra.gs = gs;
-      ra.ng = L->ng;
-      ra.Kc = L->Kc;
-      ra.qo = (uint32_t*)qo;
-      ra.so = (uint16_t*)so;
-      ra.zo = (uint16_t*)zo;
-      if (!cuda(launch_repack(ra, st), LLMOC_ERR_CUDA)) break;
+      ra.ng = ng;
+      ra.nb = L->nb;
+      ra.fl = L->fl;
+      ra.gptq = !awq;
+      ra.out = (uint32_t*)at;
+      if (!cuda(launch_lin_pack(ra, st), LLMOC_ERR_CUDA)) break;
       note_launches(1);
-      const size_t t16 = (size_t)(v.M + 15) / 16;
-      qo += t16 * L->Kc * 512;
-      so += t16 * L->ng * 32;
-      if (zo) zo += t16 * L->ng * 32;
+      at += (size_t)((v.M + 15) / 16) * tile_bytes;
     }
     if (rc != LLMOC_OK) break;
-    const size_t nrow = (size_t)L->mt * L->ng;
-    if (!cuda(launch_pair_rows((uint16_t*)L->s, nrow, st), LLMOC_ERR_CUDA)) break;
-    if (L->z && !cuda(launch_pair_rows((uint16_t*)L->z, nrow, st), LLMOC_ERR_CUDA)) break;
-    note_launches(L->z ? 2 : 1);
     cuda(cudaStreamSynchronize(st), LLMOC_ERR_CUDA);
   } while (false);
   if (st) {
@@ -266,14 +252,10 @@ llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* L, const uint16_
   OnDevice od(L->device);
   if (!od.ok) return no_device(who, L->device);
   LinArgs a{};
-  a.q = L->q;
-  a.s = L->s;
-  a.z = L->z;
+  a.q = L->arena;
   a.M = L->M;
   a.K = L->K;
-  a.Kc = L->Kc;
-  a.ng = L->ng;
-  a.gs = L->gs;
+  a.nb = L->nb;
   a.mt = L->mt;
   a.zp = L->zp;
   a.X = (const __nv_bfloat16*)X;
@@ -285,7 +267,7 @@ llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* L, const uint16_
   a.ldy = ldy;
   a.y_f32 = y_dtype == LLMOC_DTYPE_F32;
   a.x_vec = aligned(X, 16) && ldx % 8 == 0;
-  return launched(launch_linear(a, L->awq, (cudaStream_t)stream), who, 1);
+  return launched(launch_linear(a, L->fl, L->awq, (cudaStream_t)stream), who, 1);
 }
 
 // ------------------------------------------------------------------- norms

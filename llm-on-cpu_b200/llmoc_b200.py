@@ -375,30 +375,48 @@ def quantize_awq_sym(W, M: int, K: int, gs: int, bf16_scale: bool, q, scales, st
 # from them, and a tensor of another device, type or shape is refused here,
 # before the library sees its address.
 
-_DT = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
+_DT = {}  # torch.dtype -> LLMOC_DTYPE_*, filled on first use (this module does not import torch)
 
 
 def _dtype(x, what: str) -> int:
-    d = _DT.get(str(x.dtype))
+    d = _DT.get(x.dtype)
     if d is None:
-        raise LlmocError(f"{what}: {x.dtype} is not supported (bfloat16 or float32)")
+        d = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}.get(str(x.dtype))
+        if d is None:
+            raise LlmocError(f"{what}: {x.dtype} is not supported (bfloat16 or float32)")
+        _DT[x.dtype] = d
     return d
+
+
+_KINDS = ("torch.float32", "torch.int32", "torch.uint8")
+_KIND = {}
+
+
+def _kind(x) -> int:
+    """Index of the tensor's type in _KINDS (-1: another)."""
+    k = _KIND.get(x.dtype)
+    if k is None:
+        k = _KIND[x.dtype] = _KINDS.index(str(x.dtype)) if str(x.dtype) in _KINDS else -1
+    return k
 
 
 def _device(x, device: int, what: str) -> int:
     """The address of a cuda:`device` tensor."""
-    if x.device.type != "cuda" or x.device.index != device:
+    if x.get_device() != device:
         raise LlmocError(f"{what} is on {x.device}, not on cuda:{device}")
     return x.data_ptr()
 
 
 def _rows(x, rows: int, cols: int, device: int, what: str):
     """(address, row stride) of a [>= rows, cols] tensor with adjacent columns."""
-    if x.dim() != 2 or x.shape[0] < rows or x.shape[1] != cols:
-        raise LlmocError(f"{what}: shape {tuple(x.shape)}, not [{rows}, {cols}]")
-    if cols > 1 and x.stride(1) != 1:
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 2 or shape[0] < rows or shape[1] != cols:
+        raise LlmocError(f"{what}: shape {tuple(shape)}, not [{rows}, {cols}]")
+    if stride[1] != 1 and cols > 1:
         raise LlmocError(f"{what}: columns are not adjacent in memory")
-    return _device(x, device, what), x.stride(0) if rows > 1 else max(x.stride(0), cols)
+    if x.get_device() != device:
+        raise LlmocError(f"{what} is on {x.device}, not on cuda:{device}")
+    return x.data_ptr(), stride[0] if rows > 1 else max(stride[0], cols)
 
 
 class Int4Linear:
@@ -422,16 +440,17 @@ class Int4Linear:
         """Y[T, M] (bf16 or fp32) = X[T, K] (bf16) . W^T (+ R[T, M] bf16; R may be Y)."""
         if self.handle is None:
             raise LlmocError("llmoc_int4_linear_forward: the weights are closed")
-        if T <= 0:
-            check(OK if T == 0 else 1, "llmoc_int4_linear_forward: negative T")
+        if T == 0:
             return
-        x, ldx = _rows(X, T, self.K, self.device, "X")
-        y, ldy = _rows(Y, T, self.M, self.device, "Y")
-        r, ldr = _rows(R, T, self.M, self.device, "R") if R is not None else (None, 0)
+        dev = self.device
+        x, ldx = _rows(X, T, self.K, dev, "X")
+        y, ldy = _rows(Y, T, self.M, dev, "Y")
+        r, ldr = (None, 0) if R is None else _rows(R, T, self.M, dev, "R")
         if _dtype(X, "X") != DTYPE_BF16 or (R is not None and _dtype(R, "R") != DTYPE_BF16):
             raise LlmocError("llmoc_int4_linear_forward: X and R are bfloat16")
-        check(lib.llmoc_int4_linear_forward(self.handle, x, ldx, T, r, ldr, y, ldy, _dtype(Y, "Y"),
-                                            stream_ptr(stream)), "llmoc_int4_linear_forward")
+        st = lib.llmoc_int4_linear_forward(self.handle, x, ldx, T, r, ldr, y, ldy, _dtype(Y, "Y"), stream_ptr(stream))
+        if st:
+            check(st, "llmoc_int4_linear_forward")
 
     def weight_bytes(self) -> int:
         return int(lib.llmoc_int4_linear_weight_bytes(self.handle))
@@ -473,18 +492,23 @@ class ResidualNorm:
                              _dtype(self._keep[0], "norm weight") if self._keep else DTYPE_F32, at(post_weight),
                              at(post_bias), at(pre_weight), at(pre_bias), weight_offset, eps, block_scale,
                              residual_scale, self.ACTS[gate_act])
+        self._desc = C.byref(self.desc)
 
     def io(self, T: int, block, residual, residual_out, norm_out, gate) -> NormIO:
         H, dev = self.hidden, self.device
-        (b, ldb), (r, ldr), (ro, ldro), (no, ldno) = [
-            (None, 0) if x is None else _rows(x, T, H, dev, what)
-            for x, what in ((block, "block"), (residual, "residual"), (residual_out, "residual_out"),
-                            (norm_out, "norm_out"))]
-        rdt = DTYPE_BF16
-        if residual is not None or residual_out is not None:
-            rdt = _dtype(residual if residual is not None else residual_out, "residual")
-            if residual is not None and residual_out is not None and residual.dtype != residual_out.dtype:
+        b = r = ro = no = None
+        ldb = ldr = ldro = ldno = 0
+        bdt = rdt = ndt = DTYPE_BF16
+        if block is not None:
+            (b, ldb), bdt = _rows(block, T, H, dev, "block"), _dtype(block, "block")
+        if residual_out is not None:
+            (ro, ldro), rdt = _rows(residual_out, T, H, dev, "residual_out"), _dtype(residual_out, "residual_out")
+        if residual is not None:
+            (r, ldr), rdt = _rows(residual, T, H, dev, "residual"), _dtype(residual, "residual")
+            if residual_out is not None and residual.dtype != residual_out.dtype:
                 raise LlmocError("residual and residual_out differ in type")
+        if norm_out is not None:
+            (no, ldno), ndt = _rows(norm_out, T, H, dev, "norm_out"), _dtype(norm_out, "norm_out")
         g, gr, gc, gdt = None, 0, 0, DTYPE_BF16
         if gate is not None:  # [T, H], [1, H], [T, 1] or [1, 1]
             if gate.dim() != 2 or (gate.shape[0] != 1 and gate.shape[0] < T) or gate.shape[1] not in (1, H):
@@ -492,16 +516,16 @@ class ResidualNorm:
             g, gdt = _device(gate, dev, "gate"), _dtype(gate, "gate")
             gr = gate.stride(0) if gate.shape[0] > 1 else 0
             gc = gate.stride(1) if gate.shape[1] > 1 else 0
-        return NormIO(b, ldb, r, ldr, ro, ldro, no, ldno, g, gr, gc, DTYPE_BF16 if block is None else _dtype(block, "block"),
-                      rdt, DTYPE_BF16 if norm_out is None else _dtype(norm_out, "norm_out"), gdt)
+        return NormIO(b, ldb, r, ldr, ro, ldro, no, ldno, g, gr, gc, bdt, rdt, ndt, gdt)
 
     def forward(self, T: int, block, residual, residual_out, norm_out, gate=None, stream=None) -> None:
         """residual_out = residual_scale * residual + block_scale * act(gate) *
         post(block), norm_out = pre(that); any operand may be None where the
         desc needs none."""
         io = self.io(T, block, residual, residual_out, norm_out, gate)
-        check(lib.llmoc_norm_residual(C.byref(self.desc), C.byref(io), T, self.device, stream_ptr(stream)),
-              "llmoc_norm_residual")
+        st = lib.llmoc_norm_residual(self._desc, C.byref(io), T, self.device, stream_ptr(stream))
+        if st:
+            check(st, "llmoc_norm_residual")
 
 
 class BeamSearch:
@@ -510,32 +534,35 @@ class BeamSearch:
     def __init__(self, batch: int, beams: int, vocab: int, n_out: int, eos_token: int = -1, device: int = 0):
         self.desc = BeamDesc(batch, beams, vocab, n_out, eos_token)
         self.device = device
+        self._desc = C.byref(self.desc)
+        self._rows, self._kept, self._n_rows, self._vocab = (batch, beams), (batch, n_out), batch * beams, vocab
 
     def workspace_bytes(self) -> int:
         return int(lib.llmoc_beam_workspace_bytes(C.byref(self.desc)))
 
-    def _plain(self, x, shape, dtype: str, what: str):
-        if x is None:
-            return None
-        if tuple(x.shape) != shape or str(x.dtype) != dtype or not x.is_contiguous():
-            raise LlmocError(f"{what}: not a contiguous {dtype} tensor of shape {shape}")
-        return _device(x, self.device, what)
+    def _plain(self, x, shape, kind: int, what: str):
+        if x.shape != shape or _kind(x) != kind or not x.is_contiguous():
+            raise LlmocError(f"{what}: not a contiguous {_KINDS[kind]} tensor of shape {shape}")
+        if x.get_device() != self.device:
+            raise LlmocError(f"{what} is on {x.device}, not on cuda:{self.device}")
+        return x.data_ptr()
 
     def select(self, logits, scores, parent, token, out_scores, ws, ws_bytes: int, finished=None, finished_out=None,
                stream=None) -> None:
         """logits [batch * beams, vocab] (bf16 or fp32), scores [batch, beams]
         fp32, finished [batch, beams] uint8 -> parent, token (int32),
         out_scores (fp32), finished_out (uint8), all [batch, n_out]."""
-        d = self.desc
-        rows, kept = (d.batch, d.beams), (d.batch, d.n_out)
-        x, ld = _rows(logits, d.batch * d.beams, d.vocab, self.device, "logits")
-        args = (self._plain(scores, rows, "torch.float32", "scores"),
-                self._plain(finished, rows, "torch.uint8", "finished"),
-                self._plain(parent, kept, "torch.int32", "parent"), self._plain(token, kept, "torch.int32", "token"),
-                self._plain(out_scores, kept, "torch.float32", "out_scores"),
-                self._plain(finished_out, kept, "torch.uint8", "finished_out"))
-        check(lib.llmoc_beam_select(C.byref(d), x, ld, _dtype(logits, "logits"), *args, ptr(ws), ws_bytes, self.device,
-                                    stream_ptr(stream)), "llmoc_beam_select")
+        rows, kept = self._rows, self._kept
+        x, ld = _rows(logits, self._n_rows, self._vocab, self.device, "logits")
+        st = lib.llmoc_beam_select(
+            self._desc, x, ld, _dtype(logits, "logits"), self._plain(scores, rows, 0, "scores"),
+            None if finished is None else self._plain(finished, rows, 2, "finished"),
+            self._plain(parent, kept, 1, "parent"), self._plain(token, kept, 1, "token"),
+            self._plain(out_scores, kept, 0, "out_scores"),
+            None if finished_out is None else self._plain(finished_out, kept, 2, "finished_out"), ptr(ws), ws_bytes,
+            self.device, stream_ptr(stream))
+        if st:
+            check(st, "llmoc_beam_select")
 
 
 class BeamReorder:
@@ -584,11 +611,12 @@ class BeamReorder:
 
     def run(self, parent, stream=None) -> None:
         """parent [batch, n_out] int32 on the device (outside [0, beams): that row stays)."""
-        if tuple(parent.shape) != (self.batch, self.n_out) or str(parent.dtype) != "torch.int32" \
-                or not parent.is_contiguous():
+        if parent.shape != (self.batch, self.n_out) or _kind(parent) != 1 or not parent.is_contiguous():
             raise LlmocError(f"parent: not a contiguous int32 tensor of shape {(self.batch, self.n_out)}")
-        check(lib.llmoc_beam_reorder(self.tensors, self.n, _device(parent, self.device, "parent"), self.batch,
-                                     self.beams, self.n_out, self.device, stream_ptr(stream)), "llmoc_beam_reorder")
+        st = lib.llmoc_beam_reorder(self.tensors, self.n, _device(parent, self.device, "parent"), self.batch,
+                                    self.beams, self.n_out, self.device, stream_ptr(stream))
+        if st:
+            check(st, "llmoc_beam_reorder")
 
 
 def launch_count() -> int:
