@@ -41,6 +41,7 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kListMax = 512;
+constexpr int kListCut = 64;  // list length above which the closing bound is applied once more
 constexpr float kNegInf = -INFINITY;
 
 __device__ __forceinline__ float masked(float x) { return fabsf(x) <= FLT_MAX ? x : kNegInf; }
@@ -49,155 +50,396 @@ __device__ __forceinline__ uint32_t order_code(float x) {
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ unsigned long long order_code64(double x) {
-  const unsigned long long b = (unsigned long long)__double_as_longlong(x == 0. ? 0. : x);
-  return b >> 63 ? ~b : b | (1ull << 63);
-}
-__device__ __forceinline__ double from_code64(unsigned long long c) {
-  return __longlong_as_double((long long)(c >> 63 ? c & ~(1ull << 63) : ~c));
+__device__ __forceinline__ float from_code(uint32_t c) {
+  return __uint_as_float(c & 0x80000000u ? c & 0x7FFFFFFFu : ~c);
 }
 // a before b in the order "larger value, then smaller index"
 __device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
 
-template <int E, bool F32>
-__global__ void __launch_bounds__(kRowThreads) k_beam_rows(const BeamArgs a) {
+// exp(x - m) as 2^(x * kLog2e - fl(m * kLog2e)): the rounding of the constant and
+// of the product drop out of the log-sum, which the merge corrects (log_sum).
+constexpr float kLog2e = 1.44269504f;
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Above kScaleMax the products would leave fp32: exp(x - m) as 2^((x - m) * kLog2e).
+constexpr float kScaleMax = 1e38f;
+// the factor from a sum relative to m to one relative to n
+__device__ __forceinline__ float rescale(float m, float n) {
+  return exp2_fast(fabsf(m) <= kScaleMax && fabsf(n) <= kScaleMax ? m * kLog2e - n * kLog2e : (m - n) * kLog2e);
+}
+// log sum exp of a row whose largest value is m, from that sum relative to m
+__device__ __forceinline__ double log_sum(float m, double s) {
+  if (fabsf(m) > kScaleMax) return (double)m + log(s);
+  const float c = m * kLog2e;
+  return (double)m + log(s) + ((double)c - (double)m * (double)kLog2e) * 0.69314718055994531;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %5};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// A load that stays where it is written (a plain one sinks to its first use,
+// a tile later, and waits there).
+__device__ __forceinline__ uint4 ld_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float logit_at(const BeamArgs& a, long long i) {
+  return masked(a.f32 ? __ldg(reinterpret_cast<const float*>(a.logits) + i)
+                      : bf16_bits_to_f32(__ldg(reinterpret_cast<const unsigned short*>(a.logits) + i)));
+}
+
+// The slice's n_out best where more elements reach the bound than the list
+// holds (long ties, adversarial orders): the n_out-th best value by bisection on
+// the order codes (none needed when the maximum itself repeats that often),
+// then, among the elements equal to it, the last index that still belongs.
+// Reads the slice again for each step.
+__device__ __noinline__ int bisect_slice(const BeamArgs& a, long long base, int v0, int v1, float m, float* best_v,
+                                         int* best_i, int* sh_i, int* sh_cnt) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, k = a.n_out;
+  auto count = [&](auto&& in) {  // elements for which in(value, index), over the CTA
+    int mine = 0;
+    for (int c = v0 + tid; c < v1; c += kRowThreads) {
+      const float v = logit_at(a, base + c);
+      mine += v > kNegInf && in(v, c);
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    __syncthreads();
+    if (lane == 0) sh_i[warp] = mine;
+    __syncthreads();
+    int tot = 0;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) tot += sh_i[w];
+    return tot;
+  };
+  uint32_t kth = order_code(m);  // largest code that at least k elements reach
+  if (count([&](float v, int) { return order_code(v) >= kth; }) < k) {
+    kth = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = kth | (1u << bit);
+      if (count([&](float v, int) { return order_code(v) >= t; }) >= k) kth = t;
+    }
+  }
+  const int above = count([&](float v, int) { return order_code(v) > kth; });
+  int lo = v0, hi = v1 - 1;  // the smallest index up to which k - above equal ones lie
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (count([&](float v, int c) { return order_code(v) == kth && c <= mid; }) >= k - above)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  __syncthreads();
+  if (tid == 0) *sh_cnt = 0;
+  __syncthreads();
+  for (int c = v0 + tid; c < v1; c += kRowThreads) {
+    const float v = logit_at(a, base + c);
+    const uint32_t code = order_code(v);
+    if (v > kNegInf && (code > kth || (code == kth && c <= lo))) {
+      const int at = atomicAdd(sh_cnt, 1);  // k of them
+      if (at < kListMax) best_v[at] = v, best_i[at] = c;
+    }
+  }
+  __syncthreads();
+  return min(*sh_cnt, kListMax);
+}
+
+// A CTA's slice is eight warps' shares of whole tiles; a tile is 32 lanes x Q
+// pieces of eight neighbours (64 bytes a lane, in registers, each piece refilled
+// for the next tile as soon as it is used).  The warps run freely: each
+// publishes the maxima of its groups of 2^p lanes (at least n_out groups over
+// the CTA) and takes the smallest published one as its bound; an old value only
+// makes the bound weaker.  A lane's exponentials are summed relative to `ref`,
+// its first maximum, which moves only when a logit exceeds it by more than
+// kRefSlack.
+//
+// What is rare goes through one rolled loop that reads the logits again and
+// masks them (`careful`): a tile that reaches past the row's end, or one with a
+// NaN or +inf.  So the loop that runs hot stays small: inlined per piece, these
+// cases doubled the time by instruction fetches alone.  Vocabularies of fewer
+// than eight tiles (small) go through it whole, thread t taking t, t + 256, ...
+//
+// VEC: rows at 16-byte boundaries.  Else a piece comes by aligned 32-bit words,
+// each of which holds at least one byte of the row, shifted together.
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_constant__ BeamArgs a) {
+  constexpr int Q = F32 ? 2 : 4, N = 8 * Q, kTile = 32 * N;
+  constexpr int kWords = F32 ? 8 : 4;  // of a piece
+  constexpr float kRefSlack = 20.f;
   __shared__ float sh_f[kRowWarps];
   __shared__ float sh_s[kRowWarps];
-  __shared__ float sh_grp[kBeamMaxOut];
+  __shared__ uint32_t sh_grp[kBeamMaxOut];  // order codes
+  __shared__ uint32_t sh_max[kRowThreads];
   __shared__ int sh_cnt;
   __shared__ int sh_i[kRowWarps];
   __shared__ float list_v[kListMax];
   __shared__ int list_i[kListMax];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row = blockIdx.x / a.splits, sl = blockIdx.x % a.splits, k = a.n_out;
+  const int row = blockIdx.x / a.splits, sl = blockIdx.x - row * a.splits, k = a.n_out;
   grid_dep_wait();
   grid_dep_release();
-  float2* cand = a.cand + ((size_t)row * a.splits + sl) * k;
   if (!(fabsf(a.scores[row]) <= FLT_MAX) || (a.fin && a.fin[row])) return;  // the merge reads nothing of such a row
-  const int v0 = sl * a.slice, v1 = min(a.vocab, v0 + a.slice);
-  // token of value j of this thread
-  auto tok = [&](int j) { return a.vec ? v0 + ((j >> 3) * kRowThreads + tid) * 8 + (j & 7) : v0 + j * kRowThreads + tid; };
-  float x[E];
+  float2* cand = a.cand + ((size_t)row * a.splits + sl) * k;
+  const bool small = a.vocab < kRowWarps * kTile;
+  // tiles [t0, t1) of the slice, [w0, w1) of this warp
+  const int tiles = (a.vocab + kTile - 1) / kTile, each = tiles / a.splits, rest = tiles - each * a.splits;
+  auto cut = [&](int i) { return i * each + min(i, rest); };
+  const int t0 = cut(sl), t1 = cut(sl + 1);
+  const int w0 = small ? 0 : t0 + (t1 - t0) * warp / kRowWarps, w1 = small ? 1 : t0 + (t1 - t0) * (warp + 1) / kRowWarps;
   const long long base = (long long)row * a.ld;
-  if (a.vec) {
-#pragma unroll
-    for (int q = 0; q < E / 8; ++q) {
-      const int c = v0 + (q * kRowThreads + tid) * 8;
-      if (c + 8 <= v1) {
-        if (F32) {
-          const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.logits) + base + c);
-          const float4 u = __ldg(p), w = __ldg(p + 1);
-          x[q * 8] = u.x, x[q * 8 + 1] = u.y, x[q * 8 + 2] = u.z, x[q * 8 + 3] = u.w;
-          x[q * 8 + 4] = w.x, x[q * 8 + 5] = w.y, x[q * 8 + 6] = w.z, x[q * 8 + 7] = w.w;
-        } else {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + base + c));
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[q * 8 + 2 * e] = __uint_as_float(w[e] << 16);
-            x[q * 8 + 2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[q * 8 + e] = c + e >= v1 ? kNegInf
-                         : F32 ? reinterpret_cast<const float*>(a.logits)[base + c + e]
-                               : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.logits)[base + c + e]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int c = v0 + j * kRowThreads + tid;
-      x[j] = c >= v1 ? kNegInf
-             : F32   ? __ldg(reinterpret_cast<const float*>(a.logits) + base + c)
-                     : bf16_bits_to_f32(__ldg(reinterpret_cast<const unsigned short*>(a.logits) + base + c));
-    }
-  }
-  float m = kNegInf;
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    x[j] = masked(x[j]);
-    m = fmaxf(m, x[j]);
-  }
-  // maxima of groups of 2^p lanes, at least k groups over the CTA
+  const char* rowp = reinterpret_cast<const char*>(a.logits) + base * (F32 ? 4 : 2);
+  const bool shift = !VEC && !F32 && (reinterpret_cast<uintptr_t>(rowp) & 2);
+  if (tid == 0) sh_cnt = 0;
   int p = 5;
   while ((kRowThreads >> p) < k) --p;
-  float gm = m, wm;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const float other = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    m = other;
-    if (o < (1 << p)) gm = m;
-  }
-  wm = m;
   const int ng = kRowThreads >> p;
-  if ((lane & ((1 << p) - 1)) == 0 && (tid >> p) < ng) sh_grp[tid >> p] = gm;
-  if (lane == 0) sh_f[warp] = wm;
-  if (tid == 0) sh_cnt = 0;
-  __syncthreads();
-  float M = sh_f[0], bound = sh_grp[0];
+
+  uint32_t u[Q][kWords];
+  auto full = [&](int t) { return !small && (t + 1) * kTile <= a.vocab; };  // the tile lies in the row
+  auto fetch = [&](int t, int q) {
+    const char* src = rowp + (size_t)(t * kTile + (q * 32 + lane) * 8) * (F32 ? 4 : 2);
+    if (VEC) {
 #pragma unroll
-  for (int w = 1; w < kRowWarps; ++w) M = fmaxf(M, sh_f[w]);
-  for (int i = 1; i < ng; ++i) bound = fminf(bound, sh_grp[i]);
-  // sum of exponentials below the slice's max
-  float s = 0.f;
-  if (M > kNegInf) {
+      for (int h = 0; h < kWords / 4; ++h) {
+        const uint4 v = ld_once(reinterpret_cast<const uint4*>(src) + h);
+        u[q][4 * h] = v.x, u[q][4 * h + 1] = v.y, u[q][4 * h + 2] = v.z, u[q][4 * h + 3] = v.w;
+      }
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(src - (shift ? 2 : 0));
 #pragma unroll
-    for (int j = 0; j < E; ++j) s += __expf(x[j] - M);
+      for (int i = 0; i < kWords; ++i) u[q][i] = __ldg(w + i);
+      if (shift) {
+        const uint32_t last = __ldg(w + kWords);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) u[q][i] = __funnelshift_r(u[q][i], i + 1 < kWords ? u[q][i + 1] : last, 16);
+      }
+    }
+  };
+  auto value = [](const uint32_t (&w)[kWords], int e) {
+    return __uint_as_float(F32 ? w[e] : e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+  };
+  // the largest logit of the lane's tile in u; NaN are passed over
+  auto tile_max = [&]() {
+    if (F32) {
+      float v = kNegInf;
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v = fmaxf(v, value(u[q], e));
+      return v;
+    }
+    __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&u[0][0]);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) v = __hmax2(v, *reinterpret_cast<const __nv_bfloat162*>(&u[q][i]));
+    return fmaxf(__low2float(v), __high2float(v));
+  };
+  // index of this lane's element j of tile t
+  auto index = [&](int t, int j) {
+    return small ? tid + j * kRowThreads : t * kTile + ((j >> 3) * 32 + lane) * 8 + (j & 7);
+  };
+  auto masked_max = [&](int t) {
+    float v = kNegInf;
+#pragma unroll 16
+    for (int j = 0; j < N; ++j) {
+      const int i = index(t, j);
+      if (i < a.vocab) v = fmaxf(v, logit_at(a, base + i));
+    }
+    return v;
+  };
+  float m = kNegInf;                     // this lane's max
+  float ref = kNegInf, c = 0.f, s = 0.f;  // its reference, fl(ref * kLog2e), and sum
+  float bound = kNegInf;                 // at least k elements of the slice reach it
+  float shown = kNegInf;                 // the maximum published for this lane's group
+  auto publish = [&]() {
+    shown = m;
+    for (int o = 1; o < (1 << p); o <<= 1) shown = fmaxf(shown, __shfl_xor_sync(0xffffffffu, shown, o));
+    if ((lane & ((1 << p) - 1)) == 0) *const_cast<volatile uint32_t*>(&sh_grp[tid >> p]) = order_code(shown);
+  };
+  auto read_bound = [&]() {
+    const volatile uint32_t* grp = sh_grp;
+    uint32_t g = grp[lane & (ng - 1)];
+    for (int i = 32; i < ng; i += 32) g = min(g, grp[i + lane]);
+    bound = fmaxf(bound, from_code(__reduce_min_sync(0xffffffffu, g)));
+  };
+  auto move_ref = [&](float to) {
+    s = s > 0.f ? s * rescale(ref, to) : 0.f;
+    ref = to;
+    c = to * kLog2e;
+  };
+  auto take = [&](float v, int i) {
+    const int at = atomicAdd(&sh_cnt, 1);
+    if (at < kListMax) list_v[at] = v, list_i[at] = i;
+  };
+  auto careful = [&](int t, bool taken) {  // maximum, sum and (not taken yet) candidates of a tile, masked
+    const float tm = masked_max(t);
+    m = fmaxf(m, tm);
+    if (tm > ref) move_ref(tm);
+#pragma unroll 16
+    for (int j = 0; j < N; ++j) {
+      const int i = index(t, j);
+      const float v = i < a.vocab ? logit_at(a, base + i) : kNegInf;
+      if (v > kNegInf) {
+        s += exp2_fast((v - ref) * kLog2e);
+        if (v >= bound && !taken) take(v, i);
+      }
+    }
+  };
+  if (w0 < w1 && full(w0)) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) fetch(w0, q);
+    m = tile_max();
+    if (!(m <= FLT_MAX)) m = masked_max(w0);
+  } else if (w0 < w1) {
+    m = masked_max(w0);
   }
+  if (m > kNegInf) move_ref(m);
+  publish();
+  sh_max[tid] = order_code(m);
+  __syncthreads();
+  if (warp == 0) {
+    // the n_out-th largest of the 256 lanes' maxima, its upper 16 bits (all of a
+    // bf16's): eight codes a lane, bisected
+    uint32_t v[kRowWarps], kth = 0;
+#pragma unroll
+    for (int i = 0; i < kRowWarps; ++i) v[i] = sh_max[i * 32 + lane];
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t t = kth | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kRowWarps; ++i) n += v[i] >= t;
+      if (__reduce_add_sync(0xffffffffu, n) >= k) kth = t;
+    }
+    if (lane == 0) sh_max[0] = kth;
+  }
+  __syncthreads();
+  bound = sh_max[0] <= order_code(kNegInf) ? kNegInf : from_code(sh_max[0]);
+  read_bound();
+  for (int t = w0; t < w1; ++t) {
+    if (full(t)) {
+      const bool more = t + 1 < w1 && full(t + 1);
+      const float tm = tile_max();
+      if (tm > ref + kRefSlack && tm <= FLT_MAX) move_ref(tm);
+      // a branch of the whole warp: were it each lane's own, the compiler would
+      // give both sides a copy of the sums, one after the other (measured: 1.7
+      // times the exponentials)
+      const bool hit = tm >= bound && tm > kNegInf && tm <= FLT_MAX;
+      if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll 1
+        for (int q = 0; q < Q; ++q) {
+          uint32_t w[kWords];  // u[q]
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            w[i] = u[0][i];
+#pragma unroll
+            for (int r = 1; r < Q; ++r) w[i] = q == r ? u[r][i] : w[i];
+          }
+          float wm = value(w, 0);
+#pragma unroll
+          for (int e = 1; e < 8; ++e) wm = fmaxf(wm, value(w, e));
+          if (!__any_sync(0xffffffffu, hit && wm >= bound)) continue;
+#pragma unroll 1
+          for (int i = 0; i < kWords; ++i) {  // w[0] is the word at hand
+#pragma unroll
+            for (int h = 0; h < (F32 ? 1 : 2); ++h) {
+              const float v = value(w, h);
+              if (hit && v >= bound && v > kNegInf) take(v, t * kTile + (q * 32 + lane) * 8 + i * (F32 ? 1 : 2) + h);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r + 1 < kWords; ++r) w[r] = w[r + 1];
+          }
+        }
+      }
+      float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 x = fma2(make_float2(value(u[q], e), value(u[q], e + 1)), kLog2e, -c);
+          sum[e >> 1 & 1] = add2(sum[e >> 1 & 1], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+        }
+        if (more) fetch(t + 1, q);
+      }
+      const float ts = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      if (tm <= FLT_MAX) m = fmaxf(m, tm);
+      if (ts <= FLT_MAX && fabsf(ref) <= kScaleMax)
+        s += ts;
+      else  // a NaN, +inf (no candidates taken yet), or products that leave fp32
+        careful(t, tm <= FLT_MAX);
+    } else {
+      careful(t, false);
+    }
+    __syncwarp();
+    if (__any_sync(0xffffffffu, m > shown)) publish();
+    read_bound();
+  }
+  // the slice's max and sum
+  float M = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (lane == 0) sh_f[warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) M = fmaxf(M, sh_f[w]);
+  s = s > 0.f ? s * rescale(ref, M) : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) sh_s[warp] = s;
-  // what reaches the bound
-#pragma unroll
-  for (int j = 0; j < E; ++j)
-    if (x[j] >= bound && x[j] > kNegInf) {
-      const int at = atomicAdd(&sh_cnt, 1);
-      if (at < kListMax) list_v[at] = x[j], list_i[at] = tok(j);
-    }
-  __syncthreads();
-  if (tid == 0) {
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) t += sh_s[w];
-    a.stat[(size_t)row * a.splits + sl] = make_float2(M, t);
-  }
   int n = sh_cnt;
   if (n > kListMax) {
-    // the k-th best key by bisection: 32 value bits, then the index (smaller first)
-    uint64_t lo = 0;  // largest key with at least k elements >= it
-    for (int bit = 62; bit >= 0; --bit) {
-      const uint64_t c = lo | (1ull << bit);
-      int mine = 0;
+    n = bisect_slice(a, base, t0 * kTile, min(a.vocab, t1 * kTile), M, list_v, list_i, sh_i, &sh_cnt);
+  } else if (n > kListCut) {  // the last bound leaves few of a long list
+    read_bound();
+    constexpr int kMine = kListMax / kRowThreads;
+    float v[kMine];
+    int id[kMine];
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const uint64_t key = ((uint64_t)order_code(x[j]) << 31) | (uint32_t)(0x7FFFFFFF - tok(j));
-        mine += x[j] > kNegInf && key >= c;
-      }
-      mine = __reduce_add_sync(0xffffffffu, mine);
-      __syncthreads();
-      if (lane == 0) sh_i[warp] = mine;
-      __syncthreads();
-      int tot = 0;
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) tot += sh_i[w];
-      if (tot >= k) lo = c;
+    for (int j = 0; j < kMine; ++j) {
+      const int i = tid + j * kRowThreads;
+      v[j] = i < n ? list_v[i] : kNegInf;
+      id[j] = i < n ? list_i[i] : 0;
     }
     __syncthreads();
     if (tid == 0) sh_cnt = 0;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const uint64_t key = ((uint64_t)order_code(x[j]) << 31) | (uint32_t)(0x7FFFFFFF - tok(j));
-      if (x[j] > kNegInf && key >= lo) {
-        const int at = atomicAdd(&sh_cnt, 1);  // k of them
-        if (at < kListMax) list_v[at] = x[j], list_i[at] = tok(j);
+    for (int j = 0; j < kMine; ++j)
+      if (v[j] >= bound && v[j] > kNegInf) {
+        const int i = atomicAdd(&sh_cnt, 1);
+        list_v[i] = v[j], list_i[i] = id[j];
       }
-    }
     __syncthreads();
-    n = min(sh_cnt, kListMax);
+    n = sh_cnt;
+  } else {
+    __syncthreads();
+  }
+  if (tid == 0) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) t += sh_s[w];
+    a.stat[(size_t)row * a.splits + sl] = make_float2(M, t);
   }
   for (int i = tid; i < n; i += kRowThreads) {
     const float v = list_v[i];
@@ -212,41 +454,58 @@ __global__ void __launch_bounds__(kRowThreads) k_beam_rows(const BeamArgs a) {
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWarps = kMergeThreads / 32;
 constexpr int kMergeList = 1024;
+constexpr int kMergeMine = 8;  // entries a thread holds (the fewer-than-2048 case)
 
-__global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_constant__ BeamArgs a) {
   __shared__ double base[kBeamMaxBeams];  // score - log-sum of each live beam
   __shared__ int kind[kBeamMaxBeams];     // 0 no candidate, 1 live, 2 finished
   __shared__ double list_v[kMergeList];
   __shared__ long long list_i[kMergeList];  // beam * vocab + token
-  __shared__ unsigned long long grp[kBeamMaxOut];  // order codes
+  __shared__ double grp[kBeamMaxOut];
   __shared__ double red_v[kMergeWarps];
   __shared__ long long red_i[kMergeWarps];
   __shared__ int cnt;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x, W = a.beams, S = a.splits, k = a.n_out;
+  const int per = S * k, all = W * per;  // entries of a beam, of the sequence
+  const bool held = all <= kMergeMine * kMergeThreads;
+  const float2* cand = a.cand + (size_t)b * all;
   grid_dep_wait();
   grid_dep_release();
   if (tid == 0) cnt = 0;
-  if (tid < kBeamMaxOut) grp[tid] = 0;
+  // every load of the common case is in flight before the first is used (what a
+  // beam without candidates left in the workspace is read, not used)
+  // neighbouring entries (one beam's) go to different warps
+  auto place = [&](int i) { return i * kMergeThreads + lane * kMergeWarps + warp; };
+  float2 mine[kMergeMine];
+#pragma unroll
+  for (int i = 0; i < kMergeMine; ++i)
+    if (held && place(i) < all) mine[i] = cand[place(i)];
   for (int w = warp; w < W; w += kMergeWarps) {  // a warp per beam: its slices in lane order
     const int row = b * W + w;
+    const float2* st = a.stat + (size_t)row * S;
+    const float2 first = lane < S ? st[lane] : make_float2(kNegInf, 0.f);
     const float sc = a.scores[row];
     int kd = fabsf(sc) <= FLT_MAX ? (a.fin && a.fin[row] ? 2 : 1) : 0;
     double lse = 0;
     if (kd == 1) {
-      float M = kNegInf;
-      for (int s = lane; s < S; s += 32) M = fmaxf(M, a.stat[(size_t)row * S + s].x);
+      float M = first.x;
+      for (int s = lane + 32; s < S; s += 32) M = fmaxf(M, st[s].x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       if (M > kNegInf) {
-        double t = 0;
-        for (int s = lane; s < S; s += 32) {
-          const float2 st = a.stat[(size_t)row * S + s];
-          if (st.x > kNegInf) t += (double)st.y * exp((double)st.x - (double)M);
-        }
+        // a slice's sum from its own max to the row's; the difference of the two is
+        // that of fp32 products, formed in fp64
+        const double c = (double)(M * kLog2e);
+        auto term = [&](const float2& v) {
+          if (!(v.x > kNegInf)) return 0.;
+          return (double)v.y * (fabsf(M) > kScaleMax ? exp((double)v.x - (double)M) : exp2((double)(v.x * kLog2e) - c));
+        };
+        double t = term(first);
+        for (int s = lane + 32; s < S; s += 32) t += term(st[s]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        lse = (double)M + log(t);
+        lse = log_sum(M, t);
       } else {
         kd = 0;  // every token masked
       }
@@ -257,41 +516,65 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
     }
   }
   __syncthreads();
-  const int lists = W * S;
-  // head of list l (a slice of a beam), or of a finished beam
-  auto entry = [&](int l, int j, double* v, long long* id) {
-    const int w = l / S, s = l % S;
+  // value and place of entry i of the sequence, read as c
+  auto entry = [&](int i, const float2& c, double* v, long long* id) {
+    const int w = i / per;
     *v = -INFINITY;
     *id = 0;
     if (kind[w] == 1) {
-      const float2 c = a.cand[((size_t)(b * W + w) * S + s) * k + j];
       if (c.x > kNegInf) *v = base[w] + (double)c.x, *id = (long long)w * a.vocab + __float_as_int(c.y);
-    } else if (kind[w] == 2 && s == 0 && j == 0) {
+    } else if (kind[w] == 2 && i == w * per) {
       *v = base[w], *id = (long long)w * a.vocab + a.eos;
     }
   };
-  // bound: the smallest of the maxima of k groups of list heads, neighbouring
-  // lists (slices of one beam) in different groups
-  const int ng = min(k, lists);
-  for (int l = tid; l < lists; l += kMergeThreads) {
-    double v;
-    long long id;
-    entry(l, 0, &v, &id);
-    atomicMax(&grp[l % ng], order_code64(v));
-  }
-  __syncthreads();
-  unsigned long long lowest = grp[0];
-  for (int i = 1; i < ng; ++i) lowest = min(lowest, grp[i]);
-  const double bound = lists < k ? -INFINITY : from_code64(lowest);
-  for (int l = tid; l < lists; l += kMergeThreads)
-    for (int j = 0; j < k; ++j) {
+  // bound: the smallest of the maxima of at least k groups of threads, over all
+  // entries held, or over the heads of the slices' lists
+  double val[kMergeMine];
+  long long pos[kMergeMine];
+  double m = -INFINITY;
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kMergeMine; ++i) {
+      val[i] = -INFINITY;
+      if (place(i) < all) entry(place(i), mine[i], &val[i], &pos[i]);
+      m = fmax(m, val[i]);
+    }
+  } else {
+    for (int l = tid; l < W * S; l += kMergeThreads) {
       double v;
       long long id;
-      entry(l, j, &v, &id);
-      if (!(v >= bound) || v == -INFINITY) break;
-      const int at = atomicAdd(&cnt, 1);
-      if (at < kMergeList) list_v[at] = v, list_i[at] = id;
+      entry(l * k, cand[l * k], &v, &id);
+      m = fmax(m, v);
     }
+  }
+  int p = 5;
+  while ((kMergeThreads >> p) < k) --p;
+  for (int o = 16; o >= (32 >> p); o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const int ng = kMergeThreads >> p;
+  if (lane < (32 >> p)) grp[warp * (32 >> p) + lane] = m;
+  __syncthreads();
+  double bound = grp[lane & (ng - 1)];
+  for (int i = 32; i < ng; i += 32) bound = fmin(bound, grp[i + lane]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) bound = fmin(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+  auto take = [&](double v, long long id) {
+    if (!(v >= bound) || v == -INFINITY) return false;
+    const int at = atomicAdd(&cnt, 1);
+    if (at < kMergeList) list_v[at] = v, list_i[at] = id;
+    return true;
+  };
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kMergeMine; ++i) take(val[i], pos[i]);
+  } else {
+    for (int l = tid; l < W * S; l += kMergeThreads)
+      for (int j = 0; j < k; ++j) {
+        double v;
+        long long id;
+        entry(l * k + j, cand[l * k + j], &v, &id);
+        if (!take(v, id)) break;
+      }
+  }
   __syncthreads();
   int n = cnt;
   if (n > kMergeList) {
@@ -303,11 +586,11 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
     for (int q = 0; q < k; ++q) {
       double bv = -INFINITY;
       long long bi = 0x7FFFFFFFFFFFFFFFll;
-      for (int l = tid; l < lists; l += kMergeThreads)
+      for (int l = tid; l < W * S; l += kMergeThreads)
         for (int j = 0; j < k; ++j) {
           double v;
           long long id;
-          entry(l, j, &v, &id);
+          entry(l * k + j, cand[l * k + j], &v, &id);
           if (v == -INFINITY) break;
           if (v < pv || (v == pv && id > pi)) {
             if (v > bv || (v == bv && id < bi)) bv = v, bi = id;
@@ -356,29 +639,29 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
 
 }  // namespace
 
-// Slices of the vocabulary per row: small ones while the grid leaves SMs
-// idle, large ones (fewer lists to merge) otherwise.
-void beam_split(int batch, int beams, int vocab, int* splits, int* slice) {
-  const long long rows = (long long)batch * beams;
-  int e = 32;
-  while (e > 8 && rows * ((vocab + e * kRowThreads - 1) / (e * kRowThreads)) < 148 * 4) e /= 2;
-  *slice = e * kRowThreads;
-  *splits = (vocab + *slice - 1) / *slice;
+// Slices of the vocabulary per row, of at least eight tiles (one a warp): the
+// number that makes rounds of resident CTAs x (tiles a warp walks + what a CTA
+// costs besides, about five tiles) the smallest.
+int beam_splits(int batch, int beams, int vocab, int f32) {
+  const long long rows = (long long)batch * beams, tiles = (vocab + (f32 ? 511 : 1023)) / (f32 ? 512 : 1024);
+  const long long resident = 148 * 4, most = std::min<long long>(std::max<long long>(1, tiles / kRowWarps), 2 * resident);
+  long long best = 1, cost = -1;
+  for (long long s = 1; s <= most; ++s) {
+    const long long per = (tiles + s * kRowWarps - 1) / (s * kRowWarps);
+    const long long c = (rows * s + resident - 1) / resident * (per + 5);
+    if (cost < 0 || c < cost) best = s, cost = c;
+  }
+  return (int)best;
 }
 
 cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t st) {
   const long long ctas = (long long)a.batch * a.beams * a.splits;
   if (ctas > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
   const dim3 grid((unsigned)ctas), block(kRowThreads);
-  cudaError_t e;
-  switch (a.slice / kRowThreads) {
-    case 8: e = a.f32 ? launch_pdl(k_beam_rows<8, true>, grid, block, 0, st, a)
-                      : launch_pdl(k_beam_rows<8, false>, grid, block, 0, st, a); break;
-    case 16: e = a.f32 ? launch_pdl(k_beam_rows<16, true>, grid, block, 0, st, a)
-                       : launch_pdl(k_beam_rows<16, false>, grid, block, 0, st, a); break;
-    default: e = a.f32 ? launch_pdl(k_beam_rows<32, true>, grid, block, 0, st, a)
-                       : launch_pdl(k_beam_rows<32, false>, grid, block, 0, st, a);
-  }
+  const cudaError_t e = a.f32 ? (a.vec ? launch_pdl(k_beam_rows<true, true>, grid, block, 0, st, a)
+                                       : launch_pdl(k_beam_rows<true, false>, grid, block, 0, st, a))
+                              : (a.vec ? launch_pdl(k_beam_rows<false, true>, grid, block, 0, st, a)
+                                       : launch_pdl(k_beam_rows<false, false>, grid, block, 0, st, a));
   if (e != cudaSuccess) return e;
   return launch_pdl(k_beam_merge, dim3((unsigned)a.batch), dim3(kMergeThreads), 0, st, a);
 }

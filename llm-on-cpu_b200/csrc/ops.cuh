@@ -73,14 +73,14 @@ struct BeamArgs {
   int* token;
   float* out;
   unsigned char* fin_out;  // or null
-  int splits, slice;       // vocabulary slices per row, elements per slice
+  int splits;  // vocabulary slices per row
   int vec;                 // rows readable by 16-byte loads
   float2* cand;            // workspace [batch * beams][splits][n_out]: (logit, index bits), best first
   float2* stat;            // workspace [batch * beams][splits]: (max, sum exp(x - max))
 };
 constexpr int kBeamMaxOut = 128;
 constexpr int kBeamMaxBeams = 128;
-void beam_split(int batch, int beams, int vocab, int* splits, int* slice);
+int beam_splits(int batch, int beams, int vocab, int f32);
 cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t st);
 
 struct ReorderTensor {

@@ -452,10 +452,9 @@ static llmoc_status check_beam(const llmoc_beam_desc* d, const char* who) {
 
 size_t llmoc_beam_workspace_bytes(const llmoc_beam_desc* d) {
   if (check_beam(d, "llmoc_beam_workspace_bytes") != LLMOC_OK) return 0;
-  int splits, slice;
-  beam_split(d->batch, d->beams, d->vocab, &splits, &slice);
-  const size_t rows = (size_t)d->batch * d->beams * splits;
-  return up256(rows * d->n_out * 8) + up256(rows * 8);
+  const int splits = std::max(beam_splits(d->batch, d->beams, d->vocab, 0), beam_splits(d->batch, d->beams, d->vocab, 1));
+  const size_t lists = (size_t)d->batch * d->beams * splits;
+  return up256(lists * d->n_out * 8) + up256(lists * 8);
 }
 
 llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int64_t ld, int logits_dtype,
@@ -509,7 +508,7 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
   a.token = token;
   a.out = out_scores;
   a.fin_out = finished_out;
-  beam_split(d->batch, d->beams, d->vocab, &a.splits, &a.slice);
+  a.splits = beam_splits(d->batch, d->beams, d->vocab, a.f32);
   a.vec = vec_rows(logits, ld * (long long)es);
   const size_t lists = (size_t)rows * a.splits;
   a.cand = (float2*)workspace;
