@@ -60,13 +60,6 @@ __device__ __forceinline__ void store8(void* p, long long i, int f32, const floa
 __device__ __forceinline__ float load1(const void* p, long long i, int f32) {
   return f32 ? reinterpret_cast<const float*>(p)[i] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
-__device__ __forceinline__ void store1(void* p, long long i, int f32, float v) {
-  if (f32)
-    reinterpret_cast<float*>(p)[i] = v;
-  else
-    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
 // Sum over the G threads of a row, in a fixed order; every thread gets it.
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* sh) {
@@ -85,10 +78,28 @@ __device__ __forceinline__ float row_sum(float v, float* sh) {
 
 constexpr int kNormMinThreads = 128;  // rows of one warp share a CTA of four
 
-// VEC: eight consecutive columns per 16-byte access; else columns G apart.
-template <int G, int VPT, bool VEC>
-__global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads) k_norm(const NormArgs a) {
+// How a thread holds its columns of an operand: eight neighbours per 16-byte
+// access (kVec), all of them bf16 and kept packed until used (kBf16), or columns
+// G apart (kScalar).
+enum { kScalar = 0, kVec = 1, kBf16 = 2 };
+
+template <int MODE, int VPT>
+struct Held {
+  float v[8 * VPT];
+};
+template <int VPT>
+struct Held<kBf16, VPT> {
+  uint4 v[VPT];
+};
+
+// HOLD: every operand of a row is requested before the first reduction, so a row
+// waits for memory once.  Without, the weights are fetched where they are used,
+// which leaves registers for more rows per SM.
+template <int G, int VPT, int MODE, bool HOLD>
+__global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads, (MODE == kBf16 || !HOLD) && VPT <= 2 ? 1024 / (G > kNormMinThreads ? G : kNormMinThreads) : 1)
+    k_norm(const __grid_constant__ NormArgs a) {
   constexpr int N = 8 * VPT;
+  using Row = Held<MODE, VPT>;
   __shared__ float sh[8][32];  // one slice per reduction of a row: no second barrier between two of them
   const int tid = G > 32 ? threadIdx.x : threadIdx.x & 31;
   const int row = G > 32 ? blockIdx.x : blockIdx.x * (kNormMinThreads / 32) + (threadIdx.x >> 5);
@@ -97,44 +108,68 @@ __global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads) k_n
   if (row >= a.T) return;  // whole warps, and only where no barrier follows (G == 32)
   const int H = a.H;
   const float inv = 1.f / (float)H;
-  // column of value j
-  auto col = [&](int j) { return VEC ? ((j >> 3) * G + tid) * 8 + (j & 7) : j * G + tid; };
-  auto load = [&](const void* p, long long off, int f32, float (&v)[N], float fill) {
-    if (VEC) {
+  auto col = [&](int j) { return MODE != kScalar ? ((j >> 3) * G + tid) * 8 + (j & 7) : j * G + tid; };
+  auto inside = [&](int j) { return MODE != kScalar ? ((j >> 3) * G + tid) * 8 < H : j * G + tid < H; };
+  // columns past H are held as 0
+  auto fetch = [&](const void* p, long long off, int f32, Row& r) {
+    if constexpr (MODE == kBf16) {
+#pragma unroll
+      for (int q = 0; q < VPT; ++q)
+        r.v[q] = inside(q * 8) ? *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p) + off + col(q * 8))
+                               : make_uint4(0, 0, 0, 0);
+    } else if constexpr (MODE == kVec) {
 #pragma unroll
       for (int q = 0; q < VPT; ++q) {
-        float x[8];
-        const int c = (q * G + tid) * 8;
-        if (c < H) load8(p, off + c, f32, x);
+        float x[8] = {};
+        if (inside(q * 8)) load8(p, off + col(q * 8), f32, x);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[q * 8 + k] = c < H ? x[k] : fill;
+        for (int k = 0; k < 8; ++k) r.v[q * 8 + k] = x[k];
       }
-    } else {
+    } else if (f32) {
+      const float* src = reinterpret_cast<const float*>(p) + off + tid;
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = col(j) < H ? load1(p, off + col(j), f32) : fill;
+      for (int j = 0; j < N; ++j) r.v[j] = inside(j) ? src[j * G] : 0.f;
+    } else {
+      const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(p) + off + tid;
+#pragma unroll
+      for (int j = 0; j < N; ++j) r.v[j] = inside(j) ? __bfloat162float(src[j * G]) : 0.f;
+    }
+  };
+  auto at = [&](const Row& r, int j) {
+    if constexpr (MODE == kBf16) {
+      const uint4& u = r.v[j >> 3];
+      const uint32_t w = (j & 7) < 2 ? u.x : (j & 7) < 4 ? u.y : (j & 7) < 6 ? u.z : u.w;
+      return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+    } else {
+      return r.v[j];
     }
   };
   auto store = [&](void* p, long long off, int f32, const float (&v)[N]) {
-    if (VEC) {
+    if (MODE != kScalar) {
 #pragma unroll
       for (int q = 0; q < VPT; ++q) {
-        const int c = (q * G + tid) * 8;
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = v[q * 8 + k];
-        if (c < H) store8(p, off + c, f32, x);
+        if (inside(q * 8)) store8(p, off + col(q * 8), MODE == kBf16 ? 0 : f32, x);
       }
-    } else {
+    } else if (f32) {
+      float* dst = reinterpret_cast<float*>(p) + off + tid;
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (col(j) < H) store1(p, off + col(j), f32, v[j]);
+        if (inside(j)) dst[j * G] = v[j];
+    } else {
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p) + off + tid;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (inside(j)) dst[j * G] = __float2bfloat16_rn(v[j]);
     }
   };
-  // x = norm(x); `at` picks the reductions' shared slices.  Sums that leave
+  // x = norm(x); `si` picks the reductions' shared slices.  Sums that leave
   // fp32's range (squares of values above about 1e17) are formed again from
   // x * 2^-80, which is exact and drops out of the quotient; eps, far below an
   // ulp of such sums, becomes any small value that keeps 0 / 0 out.
-  auto normed = [&](float (&x)[N], int kind, const void* w, const void* b, int at) {
+  auto normed = [&](float (&x)[N], int kind, const void* w, const void* b, Row& hw, Row& hb, int si) {
     float eps = a.eps;
     bool shrunk = false;
     auto shrink = [&]() {
@@ -156,93 +191,117 @@ __global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads) k_n
       return row_sum<G>(s, sh[i]);
     };
     if (kind == LLMOC_NORM_LAYER) {
-      float s = sum(at);
+      float s = sum(si);
       if (!(fabsf(s) <= FLT_MAX)) {  // the same for all threads of the row
         shrink();
-        s = sum(at + 1);
+        s = sum(si + 1);
       }
       const float mean = s * inv;
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = col(j) < H ? x[j] - mean : 0.f;
+      for (int j = 0; j < N; ++j) x[j] = inside(j) ? x[j] - mean : 0.f;
     }
-    float q = squares(at + 2);
+    float q = squares(si + 2);
     if (!(q <= FLT_MAX) && !shrunk) {
       shrink();
-      q = squares(at + 3);
+      q = squares(si + 3);
     }
     const float rs = rsqrtf(q * inv + eps);
-    float v[N];
     if (w) {
-      load(w, 0, a.w_f32, v, 0.f);
+      if (!HOLD) fetch(w, 0, a.w_f32, hw);
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = x[j] * rs * (v[j] + a.w_off);
+      for (int j = 0; j < N; ++j) x[j] = x[j] * rs * (at(hw, j) + a.w_off);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] *= rs;
     }
     if (b) {
-      load(b, 0, a.w_f32, v, 0.f);
+      if (!HOLD) fetch(b, 0, a.w_f32, hb);
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] += v[j];
+      for (int j = 0; j < N; ++j) x[j] += at(hb, j);
     }
   };
-
   auto act = [&](float v) { return a.gate_sigmoid ? 1.f / (1.f + expf(-v)) : v; };
+
+  const bool post = a.block && a.post != LLMOC_NORM_NONE, pre = a.out && a.pre != LLMOC_NORM_NONE;
+  Row hx, hr, hg, pw, pb, qw, qb;
+  if (a.block) fetch(a.block, row * a.ld_block, a.block_f32, hx);
+  if (a.res) fetch(a.res, row * a.ld_res, a.res_f32, hr);
+  float g1 = 0.f;
+  if (a.gate && a.gate_col == 0) g1 = load1(a.gate, row * a.gate_row, a.gate_f32);
+  if (HOLD) {
+    if (a.gate && a.gate_col) fetch(a.gate, row * a.gate_row, a.gate_f32, hg);
+    if (post && a.post_w) fetch(a.post_w, 0, a.w_f32, pw);
+    if (post && a.post_b) fetch(a.post_b, 0, a.w_f32, pb);
+    if (pre && a.pre_w) fetch(a.pre_w, 0, a.w_f32, qw);
+    if (pre && a.pre_b) fetch(a.pre_b, 0, a.w_f32, qb);
+  }
   float r[N];
-  if (a.res)
-    load(a.res, row * a.ld_res, a.res_f32, r, 0.f);
-  else
-#pragma unroll
-    for (int j = 0; j < N; ++j) r[j] = 0.f;
   if (a.block) {
     float x[N];
-    load(a.block, row * a.ld_block, a.block_f32, x, 0.f);
-    if (a.post != LLMOC_NORM_NONE) normed(x, a.post, a.post_w, a.post_b, 0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = at(hx, j);
+    if (post) normed(x, a.post, a.post_w, a.post_b, pw, pb, 0);
+    float scale = a.block_scale;
     if (a.gate) {
-      float gt[N];
-      const long long off = row * a.gate_row;
       if (a.gate_col == 0) {  // one value a row
-        const float one = act(load1(a.gate, off, a.gate_f32));
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] *= one;
+        scale *= act(g1);
       } else {
-        load(a.gate, off, a.gate_f32, gt, 0.f);
+        if (!HOLD) fetch(a.gate, row * a.gate_row, a.gate_f32, hg);
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] *= act(gt[j]);
+        for (int j = 0; j < N; ++j) x[j] *= act(at(hg, j));
       }
     }
+    if (a.res) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) r[j] = fmaf(a.block_scale, x[j], a.res_scale * r[j]);
-  } else if (a.res_scale != 1.f) {
+      for (int j = 0; j < N; ++j) r[j] = fmaf(scale, x[j], a.res_scale * at(hr, j));
+    } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) r[j] *= a.res_scale;
+      for (int j = 0; j < N; ++j) r[j] = scale * x[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r[j] = a.res_scale * at(hr, j);
   }
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    if (col(j) >= H) r[j] = 0.f;
+    if (!inside(j)) r[j] = 0.f;
   if (a.res_out) store(a.res_out, row * a.ld_res_out, a.res_f32, r);
   if (a.out) {
-    if (a.pre != LLMOC_NORM_NONE) normed(r, a.pre, a.pre_w, a.pre_b, 4);
+    if (pre) normed(r, a.pre, a.pre_w, a.pre_b, qw, qb, 4);
     store(a.out, row * a.ld_out, a.out_f32, r);
   }
 }
 
-template <int G, int VPT>
-cudaError_t launch_g(const NormArgs& a, cudaStream_t st) {
+template <int G, int VPT, bool HOLD>
+cudaError_t launch_held(const NormArgs& a, cudaStream_t st) {
   const dim3 block(std::max(G, kNormMinThreads));
   const dim3 grid((unsigned)(G > 32 ? a.T : (a.T + 3) / 4));
-  return a.vec ? launch_pdl(k_norm<G, VPT, true>, grid, block, 0, st, a)
-               : launch_pdl(k_norm<G, VPT, false>, grid, block, 0, st, a);
+  if (!a.vec) return launch_pdl(k_norm<G, VPT, kScalar, HOLD>, grid, block, 0, st, a);
+  const bool bf16 = !(a.block && a.block_f32) && !((a.res || a.res_out) && a.res_f32) && !(a.out && a.out_f32) &&
+                    !((a.post_w || a.post_b || a.pre_w || a.pre_b) && a.w_f32) && !(a.gate && a.gate_col && a.gate_f32);
+  if (bf16) return launch_pdl(k_norm<G, VPT, kBf16, VPT < 4>, grid, block, 0, st, a);
+  return launch_pdl(k_norm<G, VPT, kVec, HOLD>, grid, block, 0, st, a);
+}
+
+// Up to two rows per SM the chain of one row decides, and its operands are all
+// held (packed bf16 ones are, in any case); more rows want more of them
+// resident.
+template <int G, int VPT>
+cudaError_t launch_g(const NormArgs& a, cudaStream_t st) {
+  if constexpr (VPT < 4)
+    if (a.T <= 2 * 148) return launch_held<G, VPT, true>(a, st);
+  return launch_held<G, VPT, false>(a, st);
 }
 
 }  // namespace
 
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
+  const bool few = !a.vec && a.T <= 2 * 148;  // single-column accesses: fewer of them a thread
   if (a.H <= 256) return launch_g<32, 1>(a, st);
   if (a.H <= 1024) return launch_g<128, 1>(a, st);
   if (a.H <= 2048) return launch_g<256, 1>(a, st);
-  if (a.H <= 4096) return launch_g<256, 2>(a, st);
-  if (a.H <= 8192) return launch_g<512, 2>(a, st);
+  if (a.H <= 4096) return few ? launch_g<512, 1>(a, st) : launch_g<256, 2>(a, st);
+  if (a.H <= 8192) return few ? launch_g<1024, 1>(a, st) : launch_g<512, 2>(a, st);
   return launch_g<512, 4>(a, st);
 }
 
