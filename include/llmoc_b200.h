@@ -346,6 +346,11 @@ LLMOC_API llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* linear
                                                  const uint16_t* R, int64_t ldr, void* Y, int64_t ldy, int y_dtype,
                                                  void* stream);
 
+/* Synchronizes `stream`, reads and clears the handle's device error word:
+ * LLMOC_ERR_TIMEOUT when one of a forward's bounded device-side waits gave up
+ * since the last such call (its outputs are then not valid), else LLMOC_OK. */
+LLMOC_API llmoc_status llmoc_int4_linear_status(llmoc_int4_linear* linear, void* stream);
+
 /* Between two blocks of a decoder (the reference's rmsnorm_w16 and vec_add
  * launches, src/hal/cuda_backend.cpp, in one pass over the rows):
  *     u  = post(block)

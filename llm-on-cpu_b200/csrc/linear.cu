@@ -465,6 +465,7 @@ cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st) {
 }
 
 cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st) {
+  if (a.T >= kLinUmmaMinT && (!awq || a.zp < 16)) return launch_linear_umma(a, fl, awq, st);
   switch (fl) {
     case 1: return awq ? launch_fl<1, true>(a, st) : launch_fl<1, false>(a, st);
     case 2: return awq ? launch_fl<2, true>(a, st) : launch_fl<2, false>(a, st);

@@ -29,6 +29,7 @@ struct LinArgs {
   long long ldy;
   int y_f32;
   int x_vec;  // X rows readable by 16-byte loads
+  int* err;   // bit 0: a bounded wait gave up
 };
 struct LinPack {
   const uint8_t* q;   // QLWC [M][K / 2]
@@ -39,6 +40,9 @@ struct LinPack {
 };
 cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st);
 cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st);
+// linear_umma.cu: the same product for tens of tokens (tcgen05)
+cudaError_t launch_linear_umma(const LinArgs& a, int fl, bool awq, cudaStream_t st);
+constexpr int kLinUmmaMinT = 9;
 
 // ---- norm.cu
 struct NormArgs {

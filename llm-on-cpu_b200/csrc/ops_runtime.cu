@@ -28,6 +28,7 @@ struct llmoc_int4_linear {
   int fl = 4;  // 32-wide blocks per packed scale group
   bool awq = true;
   char* arena = nullptr;
+  int* err = nullptr;  // device error word, behind the stream
   size_t weight_bytes = 0;
 };
 
@@ -165,8 +166,10 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
   };
   do {
     if (!cuda(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking), LLMOC_ERR_CUDA)) break;
-    if (!cuda(cudaMalloc((void**)&L->arena, L->weight_bytes), LLMOC_ERR_NO_MEMORY)) break;
+    if (!cuda(cudaMalloc((void**)&L->arena, up256(L->weight_bytes) + 256), LLMOC_ERR_NO_MEMORY)) break;
     char* at = L->arena;
+    L->err = (int*)(L->arena + up256(L->weight_bytes));
+    if (!cuda(cudaMemsetAsync(L->err, 0, 4, st), LLMOC_ERR_CUDA)) break;
     size_t need = 0;  // staging of the largest host view
     for (int i = 0; i < n_views && !on_device; ++i) {
       const size_t n = up256((size_t)views[i].M * (K / 2)) + 2 * up256((size_t)views[i].M * ng * 2);
@@ -267,7 +270,23 @@ llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* L, const uint16_
   a.ldy = ldy;
   a.y_f32 = y_dtype == LLMOC_DTYPE_F32;
   a.x_vec = aligned(X, 16) && ldx % 8 == 0;
+  a.err = L->err;
   return launched(launch_linear(a, L->fl, L->awq, (cudaStream_t)stream), who, 1);
+}
+
+llmoc_status llmoc_int4_linear_status(llmoc_int4_linear* L, void* stream) {
+  const char* who = "llmoc_int4_linear_status";
+  if (!L) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": null linear");
+  OnDevice od(L->device);
+  if (!od.ok) return no_device(who, L->device);
+  int word = 0;
+  cudaError_t e = cudaMemcpyAsync(&word, L->err, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(L->err, 0, 4, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
+  if (e != cudaSuccess) return launched(e, who, 0);
+  if (word)
+    return refuse(LLMOC_ERR_TIMEOUT, std::string(who) + ": a bounded device-side wait gave up; outputs are not valid");
+  return LLMOC_OK;
 }
 
 // ------------------------------------------------------------------- norms

@@ -171,6 +171,7 @@ _SIGS = {
     "llmoc_int4_linear_create": (_i, [C.POINTER(Int4View), _i, _i, _i, C.POINTER(_vp)]),
     "llmoc_int4_linear_destroy": (None, [_vp]),
     "llmoc_int4_linear_weight_bytes": (_sz, [_vp]),
+    "llmoc_int4_linear_status": (_i, [_vp, _vp]),
     "llmoc_int4_linear_forward": (_i, [_vp, _vp, C.c_int64, _i, _vp, C.c_int64, _vp, C.c_int64, _i, _vp]),
     "llmoc_norm_residual": (_i, [C.POINTER(NormDesc), C.POINTER(NormIO), _i, _i, _vp]),
     "llmoc_moe_block_workspace_bytes": (_sz, [_vp, _i]),
@@ -451,6 +452,10 @@ class Int4Linear:
         st = lib.llmoc_int4_linear_forward(self.handle, x, ldx, T, r, ldr, y, ldy, _dtype(Y, "Y"), stream_ptr(stream))
         if st:
             check(st, "llmoc_int4_linear_forward")
+
+    def status(self, stream=None) -> None:
+        """Synchronizes the stream; raises if a bounded wait of a forward gave up since the last call."""
+        check(lib.llmoc_int4_linear_status(self.handle, stream_ptr(stream)), "llmoc_int4_linear_status")
 
     def weight_bytes(self) -> int:
         return int(lib.llmoc_int4_linear_weight_bytes(self.handle))
