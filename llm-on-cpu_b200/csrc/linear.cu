@@ -100,7 +100,7 @@ struct LinPlan {
 // FL: 32-wide blocks per scale group (1, 2, 4); TP: token rows staged (1, or
 // NT * 8).
 template <int FL, bool AWQ, int NT, int RT, int TP>
-__global__ void __launch_bounds__(kLinThreads, NT * RT >= 6 ? 1 : 2) k_linear(const LinArgs a, const LinPlan p) {
+__global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, const LinPlan p) {
   constexpr int kBB = lin_block_bytes(FL, !AWQ);
   constexpr int GB = 2 / RT;                    // blocks in flight per tile
   constexpr int kGrp = 8 / FL;                  // scale groups per block
@@ -411,14 +411,9 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
 
 template <int FL, bool AWQ>
 cudaError_t launch_fl(const LinArgs& a, cudaStream_t st) {
-  // token blocks of up to 32, as even as multiples of 8 allow
-  const int n8 = (a.T + 7) / 8, ntb = (n8 + 3) / 4;
-  switch ((n8 + ntb - 1) / ntb) {
-    case 1: return a.T == 1 ? launch_shape<FL, AWQ, 1, 1, 1>(a, st) : launch_shape<FL, AWQ, 1, 1, 8>(a, st);
-    case 2: return launch_shape<FL, AWQ, 2, 2, 16>(a, st);
-    case 3: return launch_shape<FL, AWQ, 3, 2, 24>(a, st);
-    default: return launch_shape<FL, AWQ, 4, 2, 32>(a, st);
-  }
+  if (a.T == 1) return launch_shape<FL, AWQ, 1, 1, 1>(a, st);
+  if (a.T <= 8) return launch_shape<FL, AWQ, 1, 1, 8>(a, st);
+  return launch_shape<FL, AWQ, 2, 2, 16>(a, st);
 }
 
 // One 32-bit word of the stream per thread: words of a block (rows past M and
@@ -465,7 +460,12 @@ cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st) {
 }
 
 cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st) {
-  if (a.T >= kLinUmmaMinT && (!awq || a.zp < 16)) return launch_linear_umma(a, fl, awq, st);
+  // From 17 tokens on mma.sync, which needs the weights dequantised once per 16
+  // tokens, is slower on every shape measured (K = 4096; T = 24, groups of 128:
+  // 9.9 against 35 us at 4096 rows, 87 against 88 at 60000); at 16 tokens it is
+  // faster for wide matrices and small groups (52 against 81 us at 60000 rows, 60
+  // against 154 with groups of 32) and about equal otherwise.
+  if (a.T > 16 && (!awq || a.zp < 16)) return launch_linear_umma(a, fl, awq, st);
   switch (fl) {
     case 1: return awq ? launch_fl<1, true>(a, st) : launch_fl<1, false>(a, st);
     case 2: return awq ? launch_fl<2, true>(a, st) : launch_fl<2, false>(a, st);

@@ -4,18 +4,23 @@
 //
 // A CTA holds 128 weight rows (eight 16-row tiles of the packed stream, see
 // linear.cu) against up to 64 tokens over a share of K, in steps of 128 k.  The
-// scale belongs to a row and a group, so it cannot ride in the A operand without
-// rounding every weight; each group gets an accumulator of its own in TMEM
-// instead, drained while the next ones are computed:
-//     acc[row][t] += s[row, g] * P[row][t],                    A = q - zp, or
-//     acc[row][t] += s * P[row][t] + (z - 16 s) * xs[g][t],    A = 16 + q (GPTQ)
-// with P from the tensor core and xs the group's activation sums.  The dequantisers
-// subtract 16 + zp from the 16 + q that linear.cu explains: one instruction per
-// pair of weights, where sums and their correction cost the loaders and the
-// drain three times that.
+// A operand is q - zp (GPTQ: q - 8, and z + 8 s times the group's activation
+// sums xs is added beside), an exact integer of four bits.  The scale belongs to
+// a row and a group:
+//
+//   groups of 128 k: an accumulator in TMEM per step, drained while the next are
+//     computed,  acc[row][t] += s[row, g] * P[row][t];
+//   smaller groups: (q - zp) * s, 4 x 11 bits, as the exact sum of two bf16
+//     operands, hi + lo.  With s = s_hi + s_lo (8 + 3 bits) hi = (q - zp) * s_hi
+//     rounded, and lo = (q - zp) * s_lo + ((q - zp) * s_hi - hi) has at most 8
+//     bits: three packed instructions per pair of weights and twice the MMAs, but
+//     one drain per step.  A drain per group of 32 took twice the time (T = 37,
+//     4101 x 7264 with zeros: 51 us against 28.7 us): each waits in turn for
+//     its MMAs, its load and the accumulator's next use.
 //
 //   TMEM   [0, 256)          accumulators: one of 64 columns per issuer
-//          [256 + 64 s)      A slot s < 4: 128 rows x 128 k, bf16 pairs
+//          [256, 512)        A slots: 4 of 64 columns (128 rows x 128 k, bf16 pairs), or
+//                            2 of hi and lo
 //   shared memory: B slots (4 x N tokens x 128 k, K-major, 128-byte swizzle),
 //   and the activation sums and scales of 16 steps, which the drain reads after
 //   it has given the accumulator back.
@@ -26,9 +31,7 @@
 //                 steps ahead, the group sums from what landed, the scales
 //   warps 8..15   dequantisers, thread = weight row = TMEM lane, even and odd
 //                 steps; the words of two steps on are in flight in registers
-//   warps 16..23  drain, one lane quadrant and half of the columns each; groups in
-//                 the order (four steps, group of the step, step), so the four
-//                 issuers' accumulators are drained in turn
+//   warps 16..23  drain, one lane quadrant and half of the columns each, step by step
 //
 // K splits over the CTAs of a cluster; their partial sums meet in distributed
 // shared memory and are added in rank order.  Every wait is bounded; one that
@@ -56,7 +59,6 @@ constexpr int kUSteps = 4;   // A and B slots
 constexpr int kUSide = 16;   // slots of sums and scales
 constexpr int kUCols = 64;   // most tokens of a CTA
 constexpr int kULinThreads = 24 * 32;
-constexpr uint32_t kUOffset = 16;
 
 struct UPlan {
   int N;       // tokens of a CTA, a multiple of 16
@@ -79,14 +81,6 @@ __device__ __forceinline__ uint4 ld_words(const char* p) {
   asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-// D (+)= A[32 k] * B: two M = 128, K = 16 MMAs
-__device__ __forceinline__ void umma_ts_k32(uint32_t tmem_d, uint32_t ta, uint64_t db, uint32_t idesc) {
-  asm volatile(
-      "{\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%4], %5, %3, 1;\n\t}\n" ::"r"(tmem_d),
-      "r"(ta), "l"(db), "r"(idesc), "r"(ta + 8), "l"(db + 2));
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -94,10 +88,36 @@ __device__ __forceinline__ void u_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// tcgen05.st of 16 columns of this warp's lane quadrant
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ uint32_t bf2_mul(uint32_t x, uint32_t y) {
+  const __nv_bfloat162 r =
+      __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf2_fma(uint32_t x, uint32_t y, uint32_t z) {
+  const __nv_bfloat162 r =
+      __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y),
+              *reinterpret_cast<const __nv_bfloat162*>(&z));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf2_dup(float f) {
+  const __nv_bfloat162 r = __float2bfloat162_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 template <int FL, bool AWQ>
 __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, const UPlan p) {
   constexpr int kBB = lin_block_bytes(FL, !AWQ);
-  constexpr int kGs = 4 / FL;   // groups (accumulator uses) per step
+  constexpr bool kSplit = FL < 4;           // the scale in the A operand, as two bf16 terms
+  constexpr int kGs = 4 / FL;               // scale groups per step
+  constexpr int kASlots = kSplit ? 2 : 4;
   constexpr int kGrp = 8 / FL;  // groups per block of the stream
   extern __shared__ __align__(1024) unsigned char usm[];
   __shared__ __align__(8) uint64_t full[kUSteps], empty[kUSteps], accFull[4], accEmpty[4], done[4];
@@ -127,8 +147,15 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
 #pragma unroll
     for (int t = 0; t < 4; ++t) raw[h][t] = ld_words(src + t * 16);
   };
+  unsigned short sraw[kGs];
+  auto fetch_scales = [&](int j) {
+    const char* src = wsrc - (r16 & 7) * 60 + hi * 2 + (size_t)(j >> 1) * kBB + 2048 + (j & 1) * (kGs * 32);
+#pragma unroll
+    for (int q = 0; q < kGs; ++q) sraw[q] = __ldg(reinterpret_cast<const unsigned short*>(src + q * 32));
+  };
   const int dg = (warp - 8) >> 2;  // even or odd steps
   if (deq && dg < n) {  // the weights do not depend on the previous kernel
+    if (kSplit) fetch_scales(j0 + dg);
     fetch(0, j0 + dg);
     fetch(1, j0 + dg);
   }
@@ -174,32 +201,24 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
       const uint32_t idesc = instr_desc(128, p.N);
       const uint64_t dB = smem_desc(su32(ringB) + warp * slot_bytes);
       const uint32_t half = (uint32_t)(p.N * 128) >> 4;  // descriptor units to the second 64 k
-      const uint32_t dacc = tmem + warp * 64, ta = tmem + 256 + warp * 64;
-      uint32_t use = 0;
-      for (int j = warp; j < n && ok; j += 4) {
-        if (!mb_wait(&full[warp], (j >> 2) & 1, &abort_flag)) {
+      const uint32_t dacc = tmem + warp * 64;
+      for (int j = warp; j < n; j += 4) {
+        const uint32_t ta = tmem + 256 + (j % kASlots) * (256 / kASlots);
+        // the step's operands, and the accumulator's last use drained
+        if (!mb_wait(&full[warp], (j >> 2) & 1, &abort_flag) ||
+            (j >= 4 && !mb_wait(&accEmpty[warp], ((j >> 2) - 1) & 1, &abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-#pragma unroll
-        for (int q = 0; q < kGs; ++q, ++use) {
-          if (use >= 1 && !mb_wait(&accEmpty[warp], (use - 1) & 1, &abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (FL == 4) {
-            umma_ts_k64(dacc, ta, dB, idesc, 0);
-            umma_ts_k64(dacc, ta + 32, dB + half, idesc, 1);
-          } else if (FL == 2) {
-            umma_ts_k64(dacc, ta + 32 * q, dB + q * half, idesc, 0);
-          } else {
-            umma_ts_k32(dacc, ta + 16 * q, dB + (q >> 1) * half + (q & 1) * 4, idesc);
-          }
-          umma_commit(&accFull[warp]);
+        umma_ts_k64(dacc, ta, dB, idesc, 0);
+        umma_ts_k64(dacc, ta + 32, dB + half, idesc, 1);
+        if (kSplit) {
+          umma_ts_k64(dacc, ta + 64, dB, idesc, 1);
+          umma_ts_k64(dacc, ta + 96, dB + half, idesc, 1);
         }
-        if (ok) umma_commit(&empty[warp]);
+        umma_commit(&accFull[warp]);
+        umma_commit(&empty[warp]);
       }
       // every MMA this thread issued has completed once its `done` fires
       umma_commit(&done[warp]);
@@ -284,9 +303,7 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
     int pub = 0;  // next step to publish
     for (int j = 0; j < n; ++j) {
       const int s = j & 3;
-      // Groups of less than a step are drained across four steps, so step j - 4
-      // may free its slot only once the three after it are published: that
-      // comes before any wait.
+      // what has landed is published before any wait
       if (j >= kUSteps && !__all_sync(0xffffffffu, mb_try(&empty[s], ((j >> 2) - 1) & 1))) {
         asm volatile("cp.async.wait_all;" ::: "memory");
         while (pub < j) publish(pub++);
@@ -306,37 +323,64 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
     while (ok && pub < n) publish(pub++);
   } else if (deq) {
     const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16) + 256;
-    const uint32_t rot = 4 * hi, zp2 = (0x4180u + ((uint32_t)a.zp << 3)) * 0x10001u;  // 16 + zp, zp < 16
+    const uint32_t rot = 4 * hi, zp2 = (0x4180u + ((AWQ ? (uint32_t)a.zp : 8u) << 3)) * 0x10001u;  // 16 + zp, zp < 16
     for (int j = dg; j < n && ok; j += 2) {
-      const int s = j & 3;
-      if (j >= kUSteps) {
-        if (!warp_wait(&empty[s], ((j >> 2) - 1) & 1)) {
+      if (j >= kASlots) {  // the slot's last MMAs
+        const int o = j - kASlots;
+        if (!warp_wait(&empty[o & 3], (o >> 2) & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
       }
+      const uint32_t ta = tl + (j % kASlots) * (256 / kASlots);
+      uint32_t shi[kGs], slo[kGs];  // the groups' scales as pairs of two bf16 terms
+      if (kSplit) {
+#pragma unroll
+        for (int q = 0; q < kGs; ++q) {
+          const float f = __half2float(__ushort_as_half(sraw[q]));
+          shi[q] = bf2_dup(f);
+          slo[q] = bf2_dup(f - __uint_as_float(shi[q] << 16));
+        }
+        if (j + 2 < n) fetch_scales(j0 + j + 2);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t wd[4] = {raw[h][t].x, raw[h][t].y, raw[h][t].z, raw[h][t].w};
+        for (int kb = 0; kb < 2; ++kb) {
+          uint32_t r[16], lo[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {  // word (kb = i >> 1, kt = i & 1): k = 32 kb + 8 t + 4 kt + {0..3}
-            const uint32_t v = __funnelshift_r(wd[i], wd[i], rot);
-            const int col = (i >> 1) * 16 + 4 * t + 2 * (i & 1);
-            r[col] = nib16(v);
-            r[col + 1] = nib16(__funnelshift_r(v, v, 8));
-            if (AWQ) r[col] = bf2_sub(r[col], zp2), r[col + 1] = bf2_sub(r[col + 1], zp2);
+          for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {  // word (kb, kt): k = 32 kb + 8 t + 4 kt + {0..3}
+              const uint4& u = raw[h][t];
+              const uint32_t w = kb ? (kt ? u.w : u.z) : (kt ? u.y : u.x);
+              const uint32_t v = __funnelshift_r(w, w, rot);
+              const int col = 4 * t + 2 * kt;
+              r[col] = nib16(v);
+              r[col + 1] = nib16(__funnelshift_r(v, v, 8));
+              r[col] = bf2_sub(r[col], zp2);
+              r[col + 1] = bf2_sub(r[col + 1], zp2);
+            }
           }
+          if (kSplit) {
+            const uint32_t hi = shi[kGs == 4 ? 2 * h + kb : h], sl = slo[kGs == 4 ? 2 * h + kb : h];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const uint32_t q = r[c];
+              r[c] = bf2_mul(q, hi);
+              lo[c] = bf2_fma(q, sl, bf2_fma(q, hi, r[c] ^ 0x80008000u));
+            }
+            tmem_st16(ta + 64 + 32 * h + 16 * kb, lo);
+          }
+          tmem_st16(ta + 32 * h + 16 * kb, r);
         }
         if (j + 2 < n) fetch(h, j0 + j + 2);
-        tmem_st32(tl + 64 * s + 32 * h, r);
       }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mb_arrive(&full[s]);
+      if (lane == 0) mb_arrive(&full[j & 3]);
     }
   } else if (ncol > 0) {
     const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16) + cbeg;
@@ -344,72 +388,58 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
     float acc[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    // Accumulator uses in order (four steps, group of the step, step).  The columns
-    // come in two halves of 16; a half's load is in flight while the one before
-    // it is added, across uses.
-    struct Use {
-      int r, q, i;  // step r * 4 + i, group q
-    };
-    auto next = [&](Use u) {
-      ++u.i;
-      if (u.i == 4 || u.r * 4 + u.i >= n) {
-        u.i = 0;
-        if (++u.q == kGs) u.q = 0, ++u.r;
-      }
-      return u;
-    };
-    Use u{0, 0, 0};
+    // The columns come in two halves of 16; a half's load is in flight while the
+    // one before it is added, across steps.
     uint32_t lo[16], up[16];
     ok = warp_wait(&accFull[0], 0);
     tc_fence_after();
     if (ok) tmem_ld16_issue(tq, lo);
-    while (ok && u.r * 4 < n) {
-      const int j = u.r * 4 + u.i, at = (j & (kUSide - 1)) * kGs + u.q;
-      // pair (g, g + 8) of the row's tile
-      const int si = ((j & (kUSide - 1)) * 8 * kGs + (row >> 4) * kGs + u.q) * 16 + (row & 7) * 2 + ((row >> 3) & 1);
-      const float s = __half2float(sc[si]);
-      const float z = AWQ ? 0.f : fmaf(-(float)kUOffset, s, __half2float(zr[si]));
-      const float* x = xs + at * kUCols + cbeg;
+    for (int j = 0; ok && j < n; ++j) {
+      const int side = j & (kUSide - 1), buf = j & 3;
+      // pair (g, g + 8) of the row's tile in the step's first scale group
+      const int si = (side * 8 + (row >> 4)) * kGs * 16 + (row & 7) * 2 + ((row >> 3) & 1);
+      const float s = kSplit ? 1.f : __half2float(sc[si]);
+      const float* x = xs + side * kGs * kUCols + cbeg;
       auto add = [&](const uint32_t (&v)[16], int c0) {
 #pragma unroll
-        for (int c = 0; c < 16; c += 4) {
-          float xa[4] = {};
-          if (kSums) {
-            const float4 xv = *reinterpret_cast<const float4*>(x + c0 + c);
-            xa[0] = xv.x, xa[1] = xv.y, xa[2] = xv.z, xa[3] = xv.w;
-          }
+        for (int c = 0; c < 16; ++c)
+          acc[c0 + c] = kSplit ? acc[c0 + c] + __uint_as_float(v[c]) : fmaf(s, __uint_as_float(v[c]), acc[c0 + c]);
+        if (kSums)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float& o = acc[c0 + c + e];
-            o = fmaf(s, __uint_as_float(v[c + e]), o);
-            if (kSums) o = fmaf(z, xa[e], o);
+          for (int q = 0; q < kGs; ++q) {
+            const int sq = si + q * 16;
+            const float z = fmaf(8.f, __half2float(sc[sq]), __half2float(zr[sq]));
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) {
+              const float4 xv = *reinterpret_cast<const float4*>(x + q * kUCols + c0 + c);
+              acc[c0 + c] = fmaf(z, xv.x, acc[c0 + c]), acc[c0 + c + 1] = fmaf(z, xv.y, acc[c0 + c + 1]);
+              acc[c0 + c + 2] = fmaf(z, xv.z, acc[c0 + c + 2]), acc[c0 + c + 3] = fmaf(z, xv.w, acc[c0 + c + 3]);
+            }
           }
-        }
       };
-      const Use nu = next(u);
       tmem_ld16_wait(lo);
       if (ncol > 16) {
-        tmem_ld16_issue(tq + u.i * 64 + 16, up);
+        tmem_ld16_issue(tq + buf * 64 + 16, up);
         add(lo, 0);
         tmem_ld16_wait(up);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mb_arrive(&accEmpty[u.i]);
+      if (lane == 0) mb_arrive(&accEmpty[buf]);
       if (ncol <= 16) {
 #pragma unroll
         for (int c = 0; c < 16; ++c) up[c] = lo[c];
       }
-      if (nu.r * 4 < n) {
-        ok = warp_wait(&accFull[nu.i], (nu.r * kGs + nu.q) & 1);
+      if (j + 1 < n) {
+        const int nb = (j + 1) & 3;
+        ok = warp_wait(&accFull[nb], ((j + 1) >> 2) & 1);
         tc_fence_after();
-        if (ok) tmem_ld16_issue(tq + nu.i * 64, lo);
+        if (ok) tmem_ld16_issue(tq + nb * 64, lo);
       }
       if (ncol > 16)
         add(up, 16);
       else
         add(up, 0);
-      u = nu;
     }
     // this warp has seen every MMA of the CTA complete: the B slots are free
     if (p.c > 1) {

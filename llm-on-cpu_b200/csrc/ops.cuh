@@ -40,9 +40,8 @@ struct LinPack {
 };
 cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st);
 cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st);
-// linear_umma.cu: the same product for tens of tokens (tcgen05)
+// linear_umma.cu: the same product for tens of tokens (tcgen05); zp < 16
 cudaError_t launch_linear_umma(const LinArgs& a, int fl, bool awq, cudaStream_t st);
-constexpr int kLinUmmaMinT = 9;
 
 // ---- norm.cu
 struct NormArgs {

@@ -159,13 +159,19 @@ def test_linear_stacked_views(asym, on_device):
         at += w.M
 
 
-@pytest.mark.parametrize("zp", [1, 8, 15])
-def test_linear_zero_points(zp):
-    w = Weight(40, 128, 32, False, seed=zp, zp=zp)
+@pytest.mark.parametrize("zp", [1, 8, 15, 20, 127])
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("T", [3, 20, 70])
+def test_linear_zero_points(zp, gs, T):
+    w = Weight(40, 384, gs, False, seed=zp, zp=zp)
     lin = L.Int4Linear.create([w.view], on_device=True)
-    x = torch.randn((3, 128), generator=gen(9), device="cuda").to(BF16)
+    x = torch.randn((T, 384), generator=gen(9), device="cuda").to(BF16)
     y = x.double() @ w.w.t()
-    close(run_linear(lin, w, x, 3, F32), y, w.tol(x, y, F32))
+    # the group sums hold (16 + q) x: their roundings are those of at most 31 |x| s where the weights are smaller
+    s = w.s.double().repeat_interleave(gs, 1)[:, :384]
+    tol = w.tol(x, y, F32) + 8 * U * (x.double().abs() @ (31 * s).t())
+    close(run_linear(lin, w, x, T, F32), y, tol)
+    lin.status(stream())
 
 
 @pytest.mark.parametrize("T", [3, 12, 40])
