@@ -108,6 +108,24 @@ __device__ __forceinline__ float logit_at(const BeamArgs& a, long long i) {
                       : bf16_bits_to_f32(__ldg(reinterpret_cast<const unsigned short*>(a.logits) + i)));
 }
 
+// By one warp: v[0] = a lower bound of the k-th largest (k <= 256) of the 256
+// order codes v, its upper 16 bits (all of a bf16's code).  Eight codes a lane,
+// bisected.
+__device__ __forceinline__ void kth_of_256(uint32_t* v, int k, int lane) {
+  uint32_t c[8], kth = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = v[i * 32 + lane];
+#pragma unroll 1
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t t = kth | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += c[i] >= t;
+    if (__reduce_add_sync(0xffffffffu, n) >= k) kth = t;
+  }
+  if (lane == 0) v[0] = kth;
+}
+
 // The slice's n_out best where more elements reach the bound than the list
 // holds (long ties, adversarial orders): the n_out-th best value by bisection on
 // the order codes (none needed when the maximum itself repeats that often),
@@ -172,10 +190,10 @@ __device__ __noinline__ int bisect_slice(const BeamArgs& a, long long base, int 
 // its first maximum, which moves only when a logit exceeds it by more than
 // kRefSlack.
 //
-// What is rare goes through one rolled loop that reads the logits again and
-// masks them (`careful`): a tile that reaches past the row's end, or one with a
-// NaN or +inf.  So the loop that runs hot stays small: inlined per piece, these
-// cases doubled the time by instruction fetches alone.  Vocabularies of fewer
+// What is rare, a tile with a NaN or +inf, goes through one rolled loop that
+// reads the logits again and masks them (`careful`).  So the loop that runs hot
+// stays small: inlined per piece, these cases doubled the time by instruction
+// fetches alone.  Vocabularies of fewer
 // than eight tiles (small) go through it whole, thread t taking t, t + 256, ...
 //
 // VEC: rows at 16-byte boundaries.  Else a piece comes by aligned 32-bit words,
@@ -197,7 +215,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
   const int row = blockIdx.x / a.splits, sl = blockIdx.x - row * a.splits, k = a.n_out;
   grid_dep_wait();
   grid_dep_release();
-  if (!(fabsf(a.scores[row]) <= FLT_MAX) || (a.fin && a.fin[row])) return;  // the merge reads nothing of such a row
+  const float score = a.scores[row];
+  const unsigned char fin = a.fin ? a.fin[row] : 0;
   float2* cand = a.cand + ((size_t)row * a.splits + sl) * k;
   const bool small = a.vocab < kRowWarps * kTile;
   // tiles [t0, t1) of the slice, [w0, w1) of this warp
@@ -214,10 +233,22 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
   const int ng = kRowThreads >> p;
 
   uint32_t u[Q][kWords];
-  auto full = [&](int t) { return !small && (t + 1) * kTile <= a.vocab; };  // the tile lies in the row
   auto fetch = [&](int t, int q) {
-    const char* src = rowp + (size_t)(t * kTile + (q * 32 + lane) * 8) * (F32 ? 4 : 2);
-    if (VEC) {
+    const int i0 = t * kTile + (q * 32 + lane) * 8;
+    const char* src = rowp + (size_t)i0 * (F32 ? 4 : 2);
+    if (i0 + 8 > a.vocab) {  // past the row's end: -inf
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) u[q][i] = F32 ? 0xFF800000u : 0xFF80FF80u;
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (i0 + e < a.vocab) {
+          if (F32)
+            u[q][e] = __ldg(reinterpret_cast<const uint32_t*>(src) + e);
+          else
+            u[q][e >> 1] = __byte_perm(u[q][e >> 1], __ldg(reinterpret_cast<const unsigned short*>(src) + e),
+                                       e & 1 ? 0x5410 : 0x3254);
+        }
+    } else if (VEC) {
 #pragma unroll
       for (int h = 0; h < kWords / 4; ++h) {
         const uint4 v = ld_once(reinterpret_cast<const uint4*>(src) + h);
@@ -305,40 +336,27 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
       }
     }
   };
-  if (w0 < w1 && full(w0)) {
+  if (!small && w0 < w1)
 #pragma unroll
     for (int q = 0; q < Q; ++q) fetch(w0, q);
+  if (!(fabsf(score) <= FLT_MAX) || fin) return;  // the merge reads nothing of such a row
+  if (small) {
+    m = masked_max(0);
+  } else if (w0 < w1) {
     m = tile_max();
     if (!(m <= FLT_MAX)) m = masked_max(w0);
-  } else if (w0 < w1) {
-    m = masked_max(w0);
   }
   if (m > kNegInf) move_ref(m);
   publish();
   sh_max[tid] = order_code(m);
   __syncthreads();
-  if (warp == 0) {
-    // the n_out-th largest of the 256 lanes' maxima, its upper 16 bits (all of a
-    // bf16's): eight codes a lane, bisected
-    uint32_t v[kRowWarps], kth = 0;
-#pragma unroll
-    for (int i = 0; i < kRowWarps; ++i) v[i] = sh_max[i * 32 + lane];
-#pragma unroll 1
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t t = kth | (1u << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kRowWarps; ++i) n += v[i] >= t;
-      if (__reduce_add_sync(0xffffffffu, n) >= k) kth = t;
-    }
-    if (lane == 0) sh_max[0] = kth;
-  }
+  if (warp == 0) kth_of_256(sh_max, k, lane);
   __syncthreads();
   bound = sh_max[0] <= order_code(kNegInf) ? kNegInf : from_code(sh_max[0]);
   read_bound();
   for (int t = w0; t < w1; ++t) {
-    if (full(t)) {
-      const bool more = t + 1 < w1 && full(t + 1);
+    if (!small) {
+      const bool more = t + 1 < w1;
       const float tm = tile_max();
       if (tm > ref + kRefSlack && tm <= FLT_MAX) move_ref(tm);
       // a branch of the whole warp: were it each lane's own, the compiler would
@@ -454,6 +472,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWarps = kMergeThreads / 32;
 constexpr int kMergeList = 1024;
+constexpr int kMergeFew = 64;
 constexpr int kMergeMine = 8;  // entries a thread holds (the fewer-than-2048 case)
 
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_constant__ BeamArgs a) {
@@ -461,7 +480,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
   __shared__ int kind[kBeamMaxBeams];     // 0 no candidate, 1 live, 2 finished
   __shared__ double list_v[kMergeList];
   __shared__ long long list_i[kMergeList];  // beam * vocab + token
-  __shared__ double grp[kBeamMaxOut];
+  __shared__ uint32_t sh_max[kMergeThreads];
   __shared__ double red_v[kMergeWarps];
   __shared__ long long red_i[kMergeWarps];
   __shared__ int cnt;
@@ -494,13 +513,8 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       if (M > kNegInf) {
-        // a slice's sum from its own max to the row's; the difference of the two is
-        // that of fp32 products, formed in fp64
-        const double c = (double)(M * kLog2e);
-        auto term = [&](const float2& v) {
-          if (!(v.x > kNegInf)) return 0.;
-          return (double)v.y * (fabsf(M) > kScaleMax ? exp((double)v.x - (double)M) : exp2((double)(v.x * kLog2e) - c));
-        };
+        // a slice's sum from its own max to the row's
+        auto term = [&](const float2& v) { return v.x > kNegInf ? (double)(v.y * rescale(v.x, M)) : 0.; };
         double t = term(first);
         for (int s = lane + 32; s < S; s += 32) t += term(st[s]);
 #pragma unroll
@@ -527,8 +541,8 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
       *v = base[w], *id = (long long)w * a.vocab + a.eos;
     }
   };
-  // bound: the smallest of the maxima of at least k groups of threads, over all
-  // entries held, or over the heads of the slices' lists
+  // bound: the k-th largest of the threads' maxima, over all entries held, or over
+  // the heads of the slices' lists
   double val[kMergeMine];
   long long pos[kMergeMine];
   double m = -INFINITY;
@@ -547,16 +561,14 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
       m = fmax(m, v);
     }
   }
-  int p = 5;
-  while ((kMergeThreads >> p) < k) --p;
-  for (int o = 16; o >= (32 >> p); o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const int ng = kMergeThreads >> p;
-  if (lane < (32 >> p)) grp[warp * (32 >> p) + lane] = m;
-  __syncthreads();
-  double bound = grp[lane & (ng - 1)];
-  for (int i = 32; i < ng; i += 32) bound = fmin(bound, grp[i + lane]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) bound = fmin(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+  double bound = -INFINITY;
+  if (all > kMergeFew) {  // fewer are ranked sooner than bounded
+    sh_max[tid] = order_code(__double2float_rd(m));
+    __syncthreads();
+    if (warp == 0) kth_of_256(sh_max, k, lane);
+    __syncthreads();
+    if (sh_max[0] > order_code(kNegInf)) bound = (double)from_code(sh_max[0]);
+  }
   auto take = [&](double v, long long id) {
     if (!(v >= bound) || v == -INFINITY) return false;
     const int at = atomicAdd(&cnt, 1);
