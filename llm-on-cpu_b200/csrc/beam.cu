@@ -19,8 +19,9 @@
 //                 ties) finds its exact n_out-th best by bisection on the
 //                 (value, index) keys, which are distinct.
 //   k_beam_merge  one CTA per sequence: each beam's log-sum from its slices,
-//                 in fp64 (candidates of different beams are compared by it),
-//                 and the best of the slices' sorted lists.
+//                 summed in fp64 (candidates of different beams are compared by
+//                 it), and the best of the slices' lists, 2048 entries at a time:
+//                 a bound, what reaches it, ranked by counting.
 //
 // Order of summation is fixed by the slice and thread numbers alone, so equal
 // rows get equal bits and ties resolve by index.
@@ -471,9 +472,11 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
 
 constexpr int kMergeThreads = 256;
 constexpr int kMergeWarps = kMergeThreads / 32;
-constexpr int kMergeList = 1024;
-constexpr int kMergeFew = 64;
-constexpr int kMergeMine = 8;  // entries a thread holds (the fewer-than-2048 case)
+constexpr int kMergeFew = 64;                               // entries ranked sooner than bounded
+constexpr int kMergeMine = 8;                               // entries a thread holds at a time
+constexpr int kMergeChunk = kMergeMine * kMergeThreads;     // of the sequence
+constexpr int kMergeKept = 2 * kBeamMaxOut;                 // most entries a cut leaves
+constexpr int kMergeList = kMergeChunk + kMergeKept;        // a chunk on top of them
 
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_constant__ BeamArgs a) {
   __shared__ double base[kBeamMaxBeams];  // score - log-sum of each live beam
@@ -481,25 +484,26 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
   __shared__ double list_v[kMergeList];
   __shared__ long long list_i[kMergeList];  // beam * vocab + token
   __shared__ uint32_t sh_max[kMergeThreads];
-  __shared__ double red_v[kMergeWarps];
-  __shared__ long long red_i[kMergeWarps];
+  __shared__ int sh_n[2][kMergeWarps];
   __shared__ int cnt;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x, W = a.beams, S = a.splits, k = a.n_out;
   const int per = S * k, all = W * per;  // entries of a beam, of the sequence
-  const bool held = all <= kMergeMine * kMergeThreads;
   const float2* cand = a.cand + (size_t)b * all;
   grid_dep_wait();
   grid_dep_release();
   if (tid == 0) cnt = 0;
-  // every load of the common case is in flight before the first is used (what a
-  // beam without candidates left in the workspace is read, not used)
-  // neighbouring entries (one beam's) go to different warps
+  // neighbouring entries (one beam's) go to different warps; a chunk's loads are
+  // all in flight at once, the first chunk's before anything else (what a beam
+  // without candidates left in the workspace is read, not used)
   auto place = [&](int i) { return i * kMergeThreads + lane * kMergeWarps + warp; };
   float2 mine[kMergeMine];
+  auto fetch = [&](int from) {
 #pragma unroll
-  for (int i = 0; i < kMergeMine; ++i)
-    if (held && place(i) < all) mine[i] = cand[place(i)];
+    for (int i = 0; i < kMergeMine; ++i)
+      if (from + place(i) < all) mine[i] = cand[from + place(i)];
+  };
+  fetch(0);
   for (int w = warp; w < W; w += kMergeWarps) {  // a warp per beam: its slices in lane order
     const int row = b * W + w;
     const float2* st = a.stat + (size_t)row * S;
@@ -530,103 +534,101 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
     }
   }
   __syncthreads();
-  // value and place of entry i of the sequence, read as c
-  auto entry = [&](int i, const float2& c, double* v, long long* id) {
-    const int w = i / per;
-    *v = -INFINITY;
-    *id = 0;
-    if (kind[w] == 1) {
-      if (c.x > kNegInf) *v = base[w] + (double)c.x, *id = (long long)w * a.vocab + __float_as_int(c.y);
-    } else if (kind[w] == 2 && i == w * per) {
-      *v = base[w], *id = (long long)w * a.vocab + a.eos;
+  // cuts the list to what reaches the upper 16 bits of its k-th value's code, or,
+  // if ties leave too many, to its k best
+  auto cut = [&](int n) {
+    constexpr int kMine = (kMergeList + kMergeThreads - 1) / kMergeThreads;
+    double v[kMine];
+    long long id[kMine];
+    uint32_t c[kMine], kth = 0;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int i = tid + j * kMergeThreads;
+      v[j] = i < n ? list_v[i] : -INFINITY;
+      id[j] = i < n ? list_i[i] : 0;
+      c[j] = i < n ? order_code(__double2float_rd(v[j])) : 0;
     }
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t t = kth | (1u << bit);
+      int m = 0;
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) m += c[j] >= t;
+      m = __reduce_add_sync(0xffffffffu, m);
+      if (lane == 0) sh_n[bit & 1][warp] = m;
+      __syncthreads();
+      m = 0;
+#pragma unroll
+      for (int w = 0; w < kMergeWarps; ++w) m += sh_n[bit & 1][w];
+      if (m >= k) kth = t;
+    }
+    if (tid == 0) cnt = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      if (c[j] >= kth && c[j] > 0) {
+        const int at = atomicAdd(&cnt, 1);
+        list_v[at] = v[j], list_i[at] = id[j];
+      }
+    __syncthreads();
+    n = cnt;
+    if (n <= kMergeKept) return;
+    int rank[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int i = tid + j * kMergeThreads;
+      rank[j] = k;
+      if (i < n) {
+        v[j] = list_v[i], id[j] = list_i[i], rank[j] = 0;
+        for (int q = 0; q < n; ++q) rank[j] += list_v[q] > v[j] || (list_v[q] == v[j] && list_i[q] < id[j]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      if (rank[j] < k) list_v[rank[j]] = v[j], list_i[rank[j]] = id[j];
+    if (tid == 0) cnt = k;
+    __syncthreads();
   };
-  // bound: the k-th largest of the threads' maxima, over all entries held, or over
-  // the heads of the slices' lists
-  double val[kMergeMine];
-  long long pos[kMergeMine];
-  double m = -INFINITY;
-  if (held) {
+  double bound = -INFINITY;
+  for (int from = 0; from < all; from += kMergeChunk) {
+    double val[kMergeMine], m = -INFINITY;
+    long long pos[kMergeMine];
 #pragma unroll
     for (int i = 0; i < kMergeMine; ++i) {
-      val[i] = -INFINITY;
-      if (place(i) < all) entry(place(i), mine[i], &val[i], &pos[i]);
+      val[i] = -INFINITY, pos[i] = 0;
+      const int e = from + place(i);
+      if (e < all) {
+        const int w = e / per;
+        if (kind[w] == 1) {
+          if (mine[i].x > kNegInf)
+            val[i] = base[w] + (double)mine[i].x, pos[i] = (long long)w * a.vocab + __float_as_int(mine[i].y);
+        } else if (kind[w] == 2 && e == w * per) {
+          val[i] = base[w], pos[i] = (long long)w * a.vocab + a.eos;
+        }
+      }
       m = fmax(m, val[i]);
     }
-  } else {
-    for (int l = tid; l < W * S; l += kMergeThreads) {
-      double v;
-      long long id;
-      entry(l * k, cand[l * k], &v, &id);
-      m = fmax(m, v);
-    }
-  }
-  double bound = -INFINITY;
-  if (all > kMergeFew) {  // fewer are ranked sooner than bounded
-    sh_max[tid] = order_code(__double2float_rd(m));
-    __syncthreads();
-    if (warp == 0) kth_of_256(sh_max, k, lane);
-    __syncthreads();
-    if (sh_max[0] > order_code(kNegInf)) bound = (double)from_code(sh_max[0]);
-  }
-  auto take = [&](double v, long long id) {
-    if (!(v >= bound) || v == -INFINITY) return false;
-    const int at = atomicAdd(&cnt, 1);
-    if (at < kMergeList) list_v[at] = v, list_i[at] = id;
-    return true;
-  };
-  if (held) {
-#pragma unroll
-    for (int i = 0; i < kMergeMine; ++i) take(val[i], pos[i]);
-  } else {
-    for (int l = tid; l < W * S; l += kMergeThreads)
-      for (int j = 0; j < k; ++j) {
-        double v;
-        long long id;
-        entry(l * k + j, cand[l * k + j], &v, &id);
-        if (!take(v, id)) break;
-      }
-  }
-  __syncthreads();
-  int n = cnt;
-  if (n > kMergeList) {
-    // too many above the bound: take the best k one by one, each the best
-    // after the last taken
-    double pv = INFINITY;
-    long long pi = -1;
-    n = 0;
-    for (int q = 0; q < k; ++q) {
-      double bv = -INFINITY;
-      long long bi = 0x7FFFFFFFFFFFFFFFll;
-      for (int l = tid; l < W * S; l += kMergeThreads)
-        for (int j = 0; j < k; ++j) {
-          double v;
-          long long id;
-          entry(l * k + j, cand[l * k + j], &v, &id);
-          if (v == -INFINITY) break;
-          if (v < pv || (v == pv && id > pi)) {
-            if (v > bv || (v == bv && id < bi)) bv = v, bi = id;
-            break;  // the rest of the list comes after it
-          }
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double ov = __shfl_xor_sync(0xffffffffu, bv, o);
-        const long long oi = __shfl_xor_sync(0xffffffffu, bi, o);
-        if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
-      }
+    if (from + kMergeChunk < all) fetch(from + kMergeChunk);
+    if (all > kMergeFew) {  // the k-th largest of the threads' maxima: at least k entries reach it
+      sh_max[tid] = order_code(__double2float_rd(m));
       __syncthreads();
-      if (lane == 0) red_v[warp] = bv, red_i[warp] = bi;
+      if (warp == 0) kth_of_256(sh_max, k, lane);
       __syncthreads();
-      for (int w = 0; w < kMergeWarps; ++w)
-        if (red_v[w] > bv || (red_v[w] == bv && red_i[w] < bi)) bv = red_v[w], bi = red_i[w];
-      if (bv == -INFINITY) break;  // uniform
-      if (tid == 0) list_v[q] = bv, list_i[q] = bi;
-      pv = bv, pi = bi;
-      n = q + 1;
+      if (sh_max[0] > order_code(kNegInf)) bound = fmax(bound, (double)from_code(sh_max[0]));
     }
+#pragma unroll
+    for (int i = 0; i < kMergeMine; ++i)
+      if (val[i] >= bound && val[i] > -INFINITY) {
+        const int at = atomicAdd(&cnt, 1);
+        list_v[at] = val[i], list_i[at] = pos[i];
+      }
     __syncthreads();
+    const int n = cnt;
+    __syncthreads();
+    if (n > 2 * kMergeFew && n > k) cut(n);  // so no more than kMergeKept stay
   }
+  const int n = cnt;
   for (int i = tid; i < n; i += kMergeThreads) {
     const double v = list_v[i];
     const long long id = list_i[i];
