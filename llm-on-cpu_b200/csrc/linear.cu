@@ -358,21 +358,25 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
 }
 
 constexpr int kLinSmemMax = 100 * 1024;  // two CTAs per SM
-constexpr long long kLinBusy = 148 * 12;
 
 template <int FL, bool AWQ, int NT, int RT, int TP>
 cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
   LinPlan p{};
   const int ntb = (a.T + NT * 8 - 1) / (NT * 8);
   const int tg = (a.mt + RT - 1) / RT;
-  // Split K while the machine has fewer than 16 busy warps per SM: inside the
-  // CTA as long as its activations stay below half of its weights, then over a
-  // cluster, then inside the CTA at any price.
+  // K is split as long as every CTA stays resident at once (two per SM) and a
+  // warp keeps a block: inside the CTA while its activations stay below half of
+  // its weights, then over a cluster, then inside the CTA at any price.  A second
+  // round of CTAs costs more than the shorter slices give (T = 8, 11008 x 4096:
+  // 344 CTAs 17.5 us, 172 CTAs 10.3 us).
   int ksw = 1, c = 1;
-  auto busy = [&]() { return (long long)tg * ntb * ksw * c >= kLinBusy || a.nb < 2 * ksw * c; };
-  while (!busy() && ksw < kLinWarps && TP * ksw * 2 <= 16 * RT) ksw *= 2, ++p.lk;
-  while (!busy() && c < 8) c *= 2, ++p.lc;
-  while (!busy() && ksw < kLinWarps) ksw *= 2, ++p.lk;
+  auto fits = [&](int w, int k) {
+    const int rbt = kLinWarps / w;
+    return (long long)((tg + rbt - 1) / rbt) * ntb * k <= 2 * 148 && a.nb >= w * k;
+  };
+  while (ksw < kLinWarps && TP * ksw * 2 <= 16 * RT && fits(2 * ksw, c)) ksw *= 2, ++p.lk;
+  while (c < 8 && fits(ksw, 2 * c)) c *= 2, ++p.lc;
+  while (ksw < kLinWarps && fits(2 * ksw, c)) ksw *= 2, ++p.lk;
   const int rbt = kLinWarps / ksw;
   p.units = (tg + rbt - 1) / rbt;
   const bool split = ksw > 1 || c > 1;
