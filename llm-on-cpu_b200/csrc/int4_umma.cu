@@ -690,9 +690,11 @@ EncodeTiled tensor_map_encoder() {
   }();
   return fn;
 }
+}  // namespace
+
 // B operand: `rows` x K bf16, row stride ld elements; boxes of 64 elements
 // (128 B, the 128-byte swizzle span) x box_rows rows; out-of-bounds rows read zero.
-bool b_tensor_map(CUtensorMap* m, const void* base, int K, int rows, int ld, int box_rows) {
+bool b_tensor_map(CUtensorMap* m, const void* base, int K, int rows, long long ld, int box_rows) {
   const EncodeTiled enc = tensor_map_encoder();
   if (!enc || rows <= 0 || K <= 0 || (reinterpret_cast<uintptr_t>(base) & 15) || (ld * 2) % 16) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
@@ -703,7 +705,6 @@ bool b_tensor_map(CUtensorMap* m, const void* base, int K, int rows, int ld, int
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-}  // namespace
 
 bool build_umma_weight_maps(const ExpertDev* h, int n_exp, int inter, int hidden, int gs, bool gptq,
                             void* host_out) {

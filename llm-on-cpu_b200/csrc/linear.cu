@@ -7,8 +7,9 @@
 // weights once: M * K / 2 bytes.
 //
 // Weights are packed for this kernel (k_lin_pack): per 16-row tile a stream of
-// blocks of 256 k, each four 512-byte chunks of words (64 k: lane L's 16 bytes
-// at 16 L) followed by the block's scales (and zeros) as fp16 pairs of rows
+// blocks of 256 k, each four 512-byte chunks of words (64 k: lane (g, t)'s 16
+// bytes at 64 g + 16 (t xor g / 2), two words of row g, then two of row g + 8, a
+// word the 8 k from 8 t of one of the chunk's two 32 k) followed by the block's scales (and zeros) as fp16 pairs of rows
 // (g, g + 8).  Groups that are other multiples of 32, 64 or 128 repeat their
 // scale, so a block holds 8, 4 or 2 groups of 32, 64 or 128.
 //
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
   uint32_t sw[GB][kGrp][RT], zw[GB][kGrp][RT];
   // a tile past the end reads the last one again; its rows are not stored
   auto tile_off = [&](int r, int unit) { return r && ((unit << lr) + wt) * RT + r < a.mt ? tile_bytes : 0; };
-  const int lq = lane * 16, ls = 2048 + g * 4;
+  const int lq = (g * 4 + (t ^ ((g >> 1) & 3))) * 16, ls = 2048 + g * 4;
 
   int unit = blockIdx.x >> p.lc, slab = 0;
   Seg cur = seg_of(unit, 0);
@@ -273,10 +274,12 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
               for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                  const uint32_t v = w[r][kb * 2 + kt];
                   uint32_t f[4];
 #pragma unroll
-                  for (int h = 0; h < 4; ++h) f[h] = nib_pair(__funnelshift_r(v, v, 4 * h));
+                  for (int h = 0; h < 4; ++h) {  // rows g and g + 8, k in two halves
+                    const uint32_t v = w[r][(h & 1) * 2 + kb];
+                    f[h] = nib_pair(__funnelshift_r(v, v, 4 * (2 * kt + (h >> 1))));
+                  }
 #pragma unroll
                   for (int n = 0; n < NT; ++n) mma16816(part[r][n], f, kt ? x[n].z : x[n].x, kt ? x[n].w : x[n].y);
                 }
@@ -432,16 +435,15 @@ __global__ void k_lin_pack(const LinPack a) {
     const long long r0 = (long long)(tb / a.nb) * 16;
     uint32_t v = 0;
     if (in < 512) {
-      const int wd = in & 3, lane = (in >> 2) & 31, g = lane >> 2, t = lane & 3;
-      const int k = b * 256 + (in >> 7) * 64 + (wd >> 1) * 32 + t * 8 + (wd & 1) * 4;
-      for (int e = 0; e < 4; ++e)
-        for (int h = 0; h < 2; ++h) {
-          const long long row = r0 + g + 8 * h;
-          if (row >= a.M || k + e >= a.K) continue;
-          const uint32_t byte = a.q[(size_t)row * (a.K / 2) + ((k + e) >> 1)];
-          const uint32_t nib = e & 1 ? byte >> 4 : byte & 15;
-          v |= nib << (4 * ((e & 1) * 4 + (e >> 1) * 2 + h));
-        }
+      const int wd = in & 3, g = (in >> 4) & 7, t = ((in >> 2) & 3) ^ ((g >> 1) & 3);
+      const int k = b * 256 + (in >> 7) * 64 + (wd & 1) * 32 + t * 8;
+      const long long row = r0 + g + 8 * (wd >> 1);
+      for (int e = 0; e < 8; ++e) {
+        if (row >= a.M || k + e >= a.K) continue;
+        const uint32_t byte = a.q[(size_t)row * (a.K / 2) + ((k + e) >> 1)];
+        const uint32_t nib = e & 1 ? byte >> 4 : byte & 15;
+        v |= nib << (4 * ((e & 1) * 4 + (e >> 1)));
+      }
       v = __funnelshift_l(v, v, 3);
     } else {
       const int s = in - 512, z = s / (8 * grp), gi = s / 8 % grp, g = s % 8;

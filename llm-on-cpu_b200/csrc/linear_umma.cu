@@ -1,52 +1,61 @@
 // linear_umma.cu — dense INT4 products of tens of tokens on the 5th-generation
-// tensor cores (tcgen05.mma): exact integers times bf16 activations, fp32 group
-// sums, the group's scale applied to its fp32 sum.
+// tensor cores (tcgen05.mma): weights times bf16 activations, exact products,
+// fp32 sums.
 //
 // A CTA holds 128 weight rows (eight 16-row tiles of the packed stream, see
 // linear.cu) against up to 64 tokens over a share of K, in steps of 128 k.  The
-// A operand is q - zp (GPTQ: q - 8, and z + 8 s times the group's activation
-// sums xs is added beside), an exact integer of four bits.  The scale belongs to
-// a row and a group:
+// A operand starts from q - zp (GPTQ: q - 8, and z + 8 s times the group's
+// activation sums xs is added beside), an exact integer of four bits.  The scale
+// belongs to a row and a group:
 //
 //   groups of 128 k: an accumulator in TMEM per step, drained while the next are
-//     computed,  acc[row][t] += s[row, g] * P[row][t];
+//     computed,  acc[row][t] += s[row, g] * P[row][t]  (GPTQ: + (z + 8 s) * xs);
 //   smaller groups: (q - zp) * s, 4 x 11 bits, as the exact sum of two bf16
 //     operands, hi + lo.  With s = s_hi + s_lo (8 + 3 bits) hi = (q - zp) * s_hi
 //     rounded, and lo = (q - zp) * s_lo + ((q - zp) * s_hi - hi) has at most 8
 //     bits: three packed instructions per pair of weights and twice the MMAs, but
-//     one drain per step.  A drain per group of 32 took twice the time (T = 37,
-//     4101 x 7264 with zeros: 51 us against 28.7 us): each waits in turn for
-//     its MMAs, its load and the accumulator's next use.
+//     no scale is left to apply, so an accumulator takes two steps.  The zeros are
+//     a product like the others, in six more columns of A and B per group: z + 8 s
+//     and xs, three bf16 terms (24 bits) each, the six largest of their products.
+//     A drain per group of 32 instead took 51 us at T = 37, 4101 x 7264 with zeros,
+//     and the zeros added in the drain 28.7 us, against 26.
+//     Two steps per drain, not four: the tensor core's sums are truncated, and
+//     four steps' err by 8e-7 of the output's norm at K = 16384, two steps' by 6e-7.
 //
-//   TMEM   [0, 256)          accumulators: one of 64 columns per issuer
-//          [256, 512)        A slots: 4 of 64 columns (128 rows x 128 k, bf16 pairs), or
-//                            2 of hi and lo
-//   shared memory: B slots (4 x N tokens x 128 k, K-major, 128-byte swizzle),
-//   and the activation sums and scales of 16 steps, which the drain reads after
-//   it has given the accumulator back.
+//   TMEM   accumulators of 64 columns, one per issuer (4; small groups 2), then
+//          the A slots: 4 of 64 columns (128 rows x 128 k, bf16 pairs), or 3 of
+//          hi and lo
+//   shared memory: B slots (N tokens x 128 k, K-major, 128-byte swizzle, and the
+//          zeros' columns), the weight blocks and scales as they are stored, the
+//          activation sums of 16 steps or the zeros' columns of A
 //
-//   warps 0..3    lane 0 issues the MMAs of the steps j % 4 == warp (an MMA costs
-//                 its issuing thread about 100 cycles, so four issue in turn)
-//   warps 4..7    activations: 16-byte cp.async into the swizzled slot up to two
-//                 steps ahead, the group sums from what landed, the scales
-//   warps 8..15   dequantisers, thread = weight row = TMEM lane, even and odd
-//                 steps; the words of two steps on are in flight in registers
-//   warps 16..23  drain, one lane quadrant and half of the columns each, step by step
+//   warps 0..3    an elected lane issues the MMAs of the steps j % 4 == warp (an MMA
+//                 costs its issuing thread 75 to 100 cycles); small groups: two warps
+//   warp  4       activations by TMA (unaligned ones: warps 6, 7 with plain loads)
+//   warp  5       weights: a bulk copy per tile and block of two steps, blocks ahead
+//   warps 6, 7    GPTQ: the group sums of what landed (mma.sync with ones)
+//   warps 8..15   dequantisers, thread = weight row = TMEM lane, even and odd steps
+//   warps 16..23  drain, one lane quadrant and half of the columns each
+//
+// Loads through registers or cp.async were the bound before: an SM got 15 bytes per
+// clock of activations that all CTAs read (T = 64, 11008 x 4096: 22.8 us, now 20.1;
+// groups of 32: 42.4, now 27.8).
 //
 // K splits over the CTAs of a cluster; their partial sums meet in distributed
 // shared memory and are added in rank order.  Every wait is bounded; one that
 // gives up sets the handle's error word (llmoc_int4_linear_status) and every role
 // drains and exits.
 //
-// Why the parity waits are sound: each barrier's waiter (an issuer for its full,
-// acc-empty and slot barriers; a dequantising warp and a loader warp for a slot's
-// empty barrier; a drain warp for an accumulator's full barrier) waits for
-// every phase of it in order, and is at most one phase ahead of it.  Sums and
-// scales of step j are overwritten by step j + 16, whose loader has seen the MMAs
-// of step j + 12 complete; their issuer had waited until every drain warp gave
-// back step j + 8's accumulator, which each does after it is through with step j.
+// Why the parity waits are sound: each barrier's waiter waits for every phase of
+// it in order and is at most one phase ahead of it: a dequantising or drain warp
+// waits for each weight block, also for a first one of which it needs no step.
+// Sums of step j are overwritten by step j + 16's, whose activations have landed
+// only after the MMAs of step j + 10 completed; their issuer had waited until every
+// drain warp gave back step j + 6's accumulator, which each does after it is
+// through with step j.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "ops.cuh"
 #include "umma_dev.cuh"
@@ -55,15 +64,35 @@ namespace llmoc {
 
 namespace {
 
-constexpr int kUSteps = 4;   // A and B slots
-constexpr int kUSide = 16;   // slots of sums and scales
 constexpr int kUCols = 64;   // most tokens of a CTA
+constexpr int kUSide = 16;   // slots of activation sums (groups of 128)
 constexpr int kULinThreads = 24 * 32;
+
+template <int FL, bool AWQ>
+struct UCfg {
+  static constexpr bool kSplit = FL < 4;             // the scale in the A operand, as two bf16 terms
+  static constexpr bool kSums = !AWQ;                // activation sums are needed
+  static constexpr bool kZCols = kSums && kSplit;    // zeros as more columns of A, the sums as more of B
+  static constexpr int kGs = 4 / FL;                 // scale groups per step
+  static constexpr int kAcc = kSplit ? 2 : 4;        // accumulators, each an issuer's
+  static constexpr int kHold = kSplit ? 2 : 1;       // steps added up in an accumulator between drains
+  static constexpr int kASlots = kSplit ? 3 : 4;     // A slots
+  static constexpr int kACols = kSplit ? 128 : 64;   // TMEM columns of one
+  static constexpr int kXSlots = kZCols ? 4 : 6;     // B slots
+  static constexpr int kRing = kZCols ? 3 : 6;       // blocks of weights, two steps each
+  static constexpr int kBB = lin_block_bytes(FL, !AWQ);
+  static constexpr int kParts = kZCols ? 3 : 2;      // 64-wide parts of a B slot
+  static constexpr int kSideBytes = kZCols ? kASlots * 16384 : kSums ? kUSide * kUCols * 4 : 0;
+  static constexpr int smem(int n) { return 1024 + kXSlots * kParts * n * 128 + kSideBytes + kRing * 8 * kBB; }
+  static_assert(kAcc * 64 + kASlots * kACols <= 512, "TMEM");
+  static_assert(smem(kUCols) <= 226 * 1024, "shared memory");
+};
 
 struct UPlan {
   int N;       // tokens of a CTA, a multiple of 16
   int c;       // CTAs of a cluster, splitting K
   int steps;   // 128-wide steps of K
+  int tma;     // the activations come by TMA
 };
 
 __device__ __forceinline__ uint32_t nib16(uint32_t w) {  // (16 + q_lo, 16 + q_hi) as bf16
@@ -76,13 +105,60 @@ __device__ __forceinline__ uint32_t bf2_sub(uint32_t x, uint32_t y) {
       __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint4 ld_words(const char* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// two fp32 sums at once
+__device__ __forceinline__ uint64_t f2_pack(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+__device__ __forceinline__ uint32_t bf2_pack(float lo, float hi) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// v = v0 + v1 + v2 in bf16 terms, 24 bits: returned as their rounded values
+struct Terms {
+  float v0, v1, v2;
+};
+__device__ __forceinline__ Terms bf16_terms(float v) {
+  Terms r;
+  r.v0 = __bfloat162float(__float2bfloat16_rn(v));
+  r.v1 = __bfloat162float(__float2bfloat16_rn(v - r.v0));
+  r.v2 = v - r.v0 - r.v1;
+  return r;
+}
+// D[tmem] += A[smem] * B[smem]^T over K = 16 * ks
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, int ks) {
+  for (int i = 0; i < ks; ++i)
+    asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, 1;" ::"r"(d), "l"(da + 2 * i), "l"(db + 2 * i),
+                 "r"(idesc));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// d[0], d[1] += the sums over 16 k of tokens 2 t, 2 t + 1 (every row the same)
+__device__ __forceinline__ void mma_ones(float (&d)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(0x3F803F80u), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void u_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -107,64 +183,87 @@ __device__ __forceinline__ uint32_t bf2_fma(uint32_t x, uint32_t y, uint32_t z) 
               *reinterpret_cast<const __nv_bfloat162*>(&z));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t bf2_fms(uint32_t x, uint32_t y, uint32_t z) {  // x y - z
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y),
+                                   __hneg2(*reinterpret_cast<const __nv_bfloat162*>(&z)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ uint32_t bf2_dup(float f) {
   const __nv_bfloat162 r = __float2bfloat162_rn(f);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// C columns of this warp's lane quadrant
+template <int C>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[C]) {
+  if constexpr (C == 16)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+  return p != 0;
+}
+
 template <int FL, bool AWQ>
-__global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, const UPlan p) {
-  constexpr int kBB = lin_block_bytes(FL, !AWQ);
-  constexpr bool kSplit = FL < 4;           // the scale in the A operand, as two bf16 terms
-  constexpr int kGs = 4 / FL;               // scale groups per step
-  constexpr int kASlots = kSplit ? 2 : 4;
+__global__ void __launch_bounds__(kULinThreads, 1)
+    k_lin_umma(const LinArgs a, const UPlan p, const __grid_constant__ CUtensorMap xmap) {
+  using C = UCfg<FL, AWQ>;
+  constexpr bool kSplit = C::kSplit, kSums = C::kSums, kZCols = C::kZCols;
+  constexpr int kGs = C::kGs, kBB = C::kBB, kAcc = C::kAcc, kASlots = C::kASlots, kXSlots = C::kXSlots, kRing = C::kRing;
   constexpr int kGrp = 8 / FL;  // groups per block of the stream
   extern __shared__ __align__(1024) unsigned char usm[];
-  __shared__ __align__(8) uint64_t full[kUSteps], empty[kUSteps], accFull[4], accEmpty[4], done[4];
+  __shared__ __align__(8) uint64_t xFull[kXSlots], full[kXSlots], empty[kXSlots], wFull[kRing], wEmpty[kRing], accFull[4],
+      accEmpty[4], done[4];
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
+  const int half_bytes = p.N * 128, slot_bytes = half_bytes * C::kParts;  // 64-wide parts of a B slot
   unsigned char* ringB = usm + ((1024 - (su32(usm) & 1023)) & 1023);
-  float* xs = reinterpret_cast<float*>(ringB + kUSteps * p.N * 256);     // [kUSide][kGs][kUCols]
-  __half* sc = reinterpret_cast<__half*>(xs + kUSide * kGs * kUCols);  // [kUSide][8 tiles][kGs][8 pairs]
-  __half* zr = sc + kUSide * kGs * 128;                                // the same (GPTQ)
+  unsigned char* side = ringB + kXSlots * slot_bytes;
+  unsigned char* ringZ = side;                         // small groups: [kASlots][128 rows][128 bytes]
+  float* xs = reinterpret_cast<float*>(side);          // groups of 128: [kUSide][kUCols]
+  unsigned char* ringW = side + C::kSideBytes;         // [kRing][8 tiles][kBB]
   auto warp_wait = [&](uint64_t* b, uint32_t par) {  // by a whole warp
     return __all_sync(0xffffffffu, mb_wait(b, par, &abort_flag)) != 0;
   };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, quad = warp & 3;
   const int rank = blockIdx.x % p.c, unit = blockIdx.x / p.c, tok0 = blockIdx.y * kUCols;
   const int j0 = p.steps * rank / p.c, n = p.steps * (rank + 1) / p.c - j0;  // this CTA's steps
-  constexpr bool kSums = !AWQ;
-  const int slot_bytes = p.N * 256;                                          // two 64-wide halves
+  const int b0 = j0 >> 1, nblk = ((j0 + n + 1) >> 1) - b0;                   // and blocks of the stream
   const size_t tile_bytes = (size_t)a.nb * kBB;
+  // the steps after which an accumulator is drained: every kHold-th of its issuer's,
+  // the issuers' in turn, and its last
+  auto drained = [&](int j) { return !kSplit || (j / kAcc + j) % C::kHold == 0 || j + kAcc >= n; };
   const int halves = p.N > 16 ? 2 : 1;  // drain warps per quadrant with columns
-  // word pieces of this dequantiser's row: 64 bytes of every chunk of its tile
-  const bool deq = warp >= 8 && warp < 16;
-  const int r16 = lane & 15, hi = r16 >> 3;
-  const char* wsrc = a.q + (size_t)min(unit * 8 + 2 * quad + (lane >> 4), a.mt - 1) * tile_bytes + (r16 & 7) * 64;
-  uint4 raw[2][4];
-  auto fetch = [&](int h, int j) {  // half h of step j
-    const char* src = wsrc + (size_t)(j >> 1) * kBB + ((j & 1) * 2 + h) * 512;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) raw[h][t] = ld_words(src + t * 16);
-  };
-  unsigned short sraw[kGs];
-  auto fetch_scales = [&](int j) {
-    const char* src = wsrc - (r16 & 7) * 60 + hi * 2 + (size_t)(j >> 1) * kBB + 2048 + (j & 1) * (kGs * 32);
-#pragma unroll
-    for (int q = 0; q < kGs; ++q) sraw[q] = __ldg(reinterpret_cast<const unsigned short*>(src + q * 32));
-  };
-  const int dg = (warp - 8) >> 2;  // even or odd steps
-  if (deq && dg < n) {  // the weights do not depend on the previous kernel
-    if (kSplit) fetch_scales(j0 + dg);
-    fetch(0, j0 + dg);
-    fetch(1, j0 + dg);
-  }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kUSteps; ++s) {
-      mb_init(&full[s], 8);  // four dequantising warps, four loader warps
+    for (int s = 0; s < kXSlots; ++s) {
+      mb_init(&xFull[s], 1);
+      mb_init(&full[s], 4 + (p.tma && !kSums ? 0 : 2));  // four dequantising warps, the activation warps
       mb_init(&empty[s], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kRing; ++i) {
+      mb_init(&wFull[i], 1);
+      mb_init(&wEmpty[i], 8 + (kSplit ? 0 : 4 * halves));  // the dequantising warps, the drain warps
+    }
+    for (int i = 0; i < kAcc; ++i) {
       mb_init(&accFull[i], 1);
       mb_init(&accEmpty[i], 4 * halves);
       mb_init(&done[i], 1);
@@ -180,45 +279,56 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
+  bool ok = true;
+  auto load_block = [&](int i) {  // by the weight warp: lanes 0..7, a tile each
+    const int slot = i % kRing;
+    if (lane == 0) mb_expect(&wFull[slot], 8 * kBB);
+    __syncwarp();
+    if (lane < 8)
+      bulk_g2s(su32(ringW) + (slot * 8 + lane) * kBB,
+               a.q + (size_t)min(unit * 8 + lane, a.mt - 1) * tile_bytes + (size_t)(b0 + i) * kBB, kBB, &wFull[slot]);
+  };
+  if (warp == 5)  // the weights do not depend on the previous kernel
+    for (int i = 0; i < kRing && i < nblk; ++i) load_block(i);
   grid_dep_wait();
   grid_dep_release();
-  bool ok = true;
-  float* red = reinterpret_cast<float*>(ringB);  // partial sums [column][row], over the B slots
-  auto store = [&](int row, int tok, float v) {
-    if (row >= a.M || tok >= a.T) return;
-    if (a.R) v += __bfloat162float(a.R[(long long)tok * a.ldr + row]);
-    if (a.y_f32)
-      reinterpret_cast<float*>(a.Y)[(long long)tok * a.ldy + row] = v;
-    else
-      reinterpret_cast<__nv_bfloat16*>(a.Y)[(long long)tok * a.ldy + row] = __float2bfloat16_rn(v);
-  };
+  float* red = reinterpret_cast<float*>(ringB);  // sums [column][row], over the B slots
   const int h2 = (warp - 16) >> 2;                            // drain: column half
   const int colw = ((p.N + 31) >> 5) << 4;                    // columns of half 0
   const int cbeg = h2 * colw, ncol = min(p.N - cbeg, colw);  // this warp's columns (16 or 32, or none)
 
   if (warp < 4) {
-    if (lane == 0) {
+    if (warp < kAcc && elect_one()) {
       const uint32_t idesc = instr_desc(128, p.N);
-      const uint64_t dB = smem_desc(su32(ringB) + warp * slot_bytes);
-      const uint32_t half = (uint32_t)(p.N * 128) >> 4;  // descriptor units to the second 64 k
+      const uint32_t half = (uint32_t)half_bytes >> 4;  // descriptor units to the next 64 k
+      const uint64_t dB0 = smem_desc(su32(ringB)), dZ = smem_desc(su32(ringZ));
       const uint32_t dacc = tmem + warp * 64;
-      for (int j = warp; j < n; j += 4) {
-        const uint32_t ta = tmem + 256 + (j % kASlots) * (256 / kASlots);
-        // the step's operands, and the accumulator's last use drained
-        if (!mb_wait(&full[warp], (j >> 2) & 1, &abort_flag) ||
-            (j >= 4 && !mb_wait(&accEmpty[warp], ((j >> 2) - 1) & 1, &abort_flag))) {
+      bool fresh = true;  // the next MMAs start a new sum
+      uint32_t drains = 0;
+      for (int j = warp; j < n; j += kAcc) {
+        const int slot = j % kXSlots, use = j / kXSlots & 1;
+        const uint32_t ta = tmem + kAcc * 64 + j % kASlots * C::kACols;
+        const uint64_t dB = dB0 + slot * (slot_bytes >> 4);
+        // the step's operands, and the accumulator's last sum drained
+        if ((p.tma && !kSums && !mb_wait(&xFull[slot], use, &abort_flag)) || !mb_wait(&full[slot], use, &abort_flag) ||
+            (fresh && drains && !mb_wait(&accEmpty[warp], (drains - 1) & 1, &abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        umma_ts_k64(dacc, ta, dB, idesc, 0);
+        umma_ts_k64(dacc, ta, dB, idesc, !fresh);
         umma_ts_k64(dacc, ta + 32, dB + half, idesc, 1);
         if (kSplit) {
           umma_ts_k64(dacc, ta + 64, dB, idesc, 1);
           umma_ts_k64(dacc, ta + 96, dB + half, idesc, 1);
         }
-        umma_commit(&accFull[warp]);
-        umma_commit(&empty[warp]);
+        if (kZCols) umma_ss(dacc, dZ + j % kASlots * 1024, dB + 2 * half, idesc, kGs / 2);
+        fresh = drained(j);
+        if (fresh) {
+          umma_commit(&accFull[warp]);
+          ++drains;
+        }
+        umma_commit(&empty[slot]);
       }
       // every MMA this thread issued has completed once its `done` fires
       umma_commit(&done[warp]);
@@ -230,242 +340,279 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
         }
     }
     __syncwarp();
-  } else if (warp < 8) {
-    const int lt = threadIdx.x - 128;  // 0..127
-    // thread's 16-byte pieces of a step: piece pc of rows r0, r0 + 8, ... (p.N / 8 of them)
-    const int pieces = p.N >> 3, pc = lt & 15, r0 = lt >> 4;
-    const uint32_t place = su32(ringB) + (pc >> 3) * (p.N * 128) + r0 * 128 + (((pc & 7) ^ r0) << 4);  // + 1024 a piece
-    const __nv_bfloat16* xsrc = a.X + (long long)(tok0 + r0) * a.ldx + pc * 8;
-    auto issue = [&](int j) {
-      const uint32_t dst = place + (j & 3) * slot_bytes;
-      if (lt < 16 * kGs) {  // the scales: kGs * 32 bytes of each tile
-        const int tile = lt / (2 * kGs), part = lt % (2 * kGs), g = j0 + j;
-        const char* src = a.q + (size_t)min(unit * 8 + tile, a.mt - 1) * tile_bytes + (size_t)(g >> 1) * kBB + 2048 +
-                          (g & 1) * (kGs * 32) + part * 16;
-        const uint32_t to = su32(sc) + (j & (kUSide - 1)) * (kGs * 256) + lt * 16;
-        cp_async16(to, src, 16);
-        if (!AWQ) cp_async16(to + kUSide * kGs * 256, src + kGrp * 32, 16);
-      }
-      const int k = (j0 + j) * 128;
-      const bool kin = k + pc * 8 < a.K;
-      if (a.x_vec) {
-        const __nv_bfloat16* src = xsrc + k;
-        const int rows = kin ? a.T - tok0 - r0 : 0;  // piece i lies in the batch: i * 8 < rows
-#pragma unroll
-        for (int i = 0; i < kUCols / 8; ++i) {
-          if (i < pieces) cp_async16(dst + i * 1024, i * 8 < rows ? src : a.X, i * 8 < rows ? 16 : 0);
-          src += 8 * a.ldx;
-        }
-      } else {
-        for (int i = 0; i < pieces; ++i) {
-          uint32_t w[4] = {0, 0, 0, 0};
-          if (kin && tok0 + r0 + i * 8 < a.T) {
-            const unsigned short* u = reinterpret_cast<const unsigned short*>(xsrc + k + i * 8 * a.ldx);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) w[q] = u[2 * q] | ((uint32_t)u[2 * q + 1] << 16);
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * 1024), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                       "r"(w[3])
-                       : "memory");
-        }
-      }
-    };
-    auto publish = [&](int j) {  // a step that has landed
-      if constexpr (kSums) {
-      const uint32_t src = place + (j & 3) * slot_bytes;
-      float* to = xs + ((j & (kUSide - 1)) * kGs + pc / (4 * FL)) * kUCols + r0;
-      float v[kUCols / 8];
-#pragma unroll
-      for (int i = 0; i < kUCols / 8; ++i) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (i < pieces)
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(src + i * 1024)
-                       : "memory");
-        v[i] = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[i] += __uint_as_float(w[q] << 16) + __uint_as_float(w[q] & 0xFFFF0000u);
-      }
-#pragma unroll
-      for (int o = 1; o < 4 * FL; o <<= 1)
-#pragma unroll
-        for (int i = 0; i < kUCols / 8; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-      if ((pc & (4 * FL - 1)) == 0)
-#pragma unroll
-        for (int i = 0; i < kUCols / 8; ++i)
-          if (i < pieces) to[i * 8] = v[i];
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mb_arrive(&full[j & 3]);
-    };
-    int pub = 0;  // next step to publish
-    for (int j = 0; j < n; ++j) {
-      const int s = j & 3;
-      // what has landed is published before any wait
-      if (j >= kUSteps && !__all_sync(0xffffffffu, mb_try(&empty[s], ((j >> 2) - 1) & 1))) {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        while (pub < j) publish(pub++);
-        if (!warp_wait(&empty[s], ((j >> 2) - 1) & 1)) {
+  } else if (warp == 4) {
+    if (p.tma && lane == 0) {
+      int j = 0;
+      for (; j < n; ++j) {
+        const int slot = j % kXSlots;
+        if (j >= kXSlots && !mb_wait(&empty[slot], (j / kXSlots - 1) & 1, &abort_flag)) {
           ok = false;
           break;
         }
+        mb_expect(&xFull[slot], 2 * half_bytes);
+        const uint32_t dst = su32(ringB) + slot * slot_bytes;
+        tma_load_2d(dst, &xmap, (j0 + j) * 128, tok0, &xFull[slot]);
+        tma_load_2d(dst + half_bytes, &xmap, (j0 + j) * 128 + 64, tok0, &xFull[slot]);
       }
-      issue(j);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (j - pub == 2) {
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-        publish(pub++);
-      }
+      if (!ok) drain_ring(xFull, kXSlots, j, 0, 1);  // no copy is in flight when the CTA leaves
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    while (ok && pub < n) publish(pub++);
-  } else if (deq) {
-    const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16) + 256;
-    const uint32_t rot = 4 * hi, zp2 = (0x4180u + ((AWQ ? (uint32_t)a.zp : 8u) << 3)) * 0x10001u;  // 16 + zp, zp < 16
+    __syncwarp();
+  } else if (warp == 5) {
+    int i = min(kRing, nblk);
+    for (; i < nblk; ++i) {
+      if (!warp_wait(&wEmpty[i % kRing], (i / kRing - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      load_block(i);
+    }
+    if (!ok) drain_ring(wFull, kRing, i, 0, 1);
+  } else if (warp < 8) {
+    // activations of 32 tokens: loaded here where TMA cannot, and their group sums
+    const int aw = warp - 6, g = lane >> 2, t = lane & 3, pc = lane & 15;
+    // The sums come from mma.sync with a row of ones, 32 k of 8 tokens per pair;
+    // every lane of a column gets them, and lane (g, t) writes those of scale group q
+    // for token 2 t + e
+    const int q = g % kGs, e = (g / kGs) & 1;
+    auto sums = [&](int j, int row0) {  // 16 tokens from row0
+      const uint32_t slot = su32(ringB) + j % kXSlots * slot_bytes;
+      const int trow = row0 + 2 * t + e;
+      float v[2][kGs][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t rows = slot + (row0 + 8 * i + (lane & 7)) * 128;
+        float d[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // 32 k: 16-byte pieces 4 k .. 4 k + 3
+          uint32_t b[4];
+          ldmatrix4(rows + (k >> 1) * half_bytes + ((((k & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b);
+          if (k % FL == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
+          mma_ones(d, b[0], b[1]);
+          mma_ones(d, b[2], b[3]);
+          if (k % FL == FL - 1) v[i][k / FL][0] = d[0], v[i][k / FL][1] = d[1];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (kGs < 4 && (g / (2 * kGs)) % 2 != i) continue;  // fewer groups: a lane writes for one of the two
+        float x = v[i][0][0];
+#pragma unroll
+        for (int c = 1; c < 2 * kGs; ++c)
+          if (c == q + e * kGs) x = v[i][c % kGs][c / kGs];
+        if (kZCols) {
+          const Terms m = bf16_terms(x);
+          const uint32_t w[3] = {bf2_pack(m.v0, m.v1), bf2_pack(m.v2, m.v0), bf2_pack(m.v1, m.v0)};
+#pragma unroll
+          for (int c = 0; c < 3; ++c) {
+            const int wi = 3 * q + c;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + 2 * half_bytes + (trow + 8 * i) * 128 +
+                                                         (((wi >> 2) ^ (trow & 7)) << 4) + (wi & 3) * 4),
+                         "r"(w[c])
+                         : "memory");
+          }
+        } else {
+          xs[(j & (kUSide - 1)) * kUCols + trow + 8 * i] = x;
+        }
+      }
+    };
+    if (kZCols)  // columns past the last group's stay zero
+      for (int s = 0; s < kXSlots; ++s)
+        for (int i = lane; i < 32 * 8 && 32 * aw + (i >> 3) < p.N; i += 32)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(su32(ringB) + s * slot_bytes + 2 * half_bytes +
+                                                                        32 * aw * 128 + i * 16),
+                       "r"(0)
+                       : "memory");
+    if (!p.tma || kSums)
+      for (int j = 0; j < n; ++j) {
+        const int slot = j % kXSlots;
+        if (p.tma) {
+          ok = warp_wait(&xFull[slot], j / kXSlots & 1);
+        } else {
+          ok = j < kXSlots || warp_wait(&empty[slot], (j / kXSlots - 1) & 1);
+          const int k = (j0 + j) * 128 + pc * 8;
+          for (int i = lane >> 4; ok && i < 32 && 32 * aw + i < p.N; i += 2) {
+            const int r = 32 * aw + i;
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (tok0 + r < a.T && k < a.K) {
+              const unsigned short* u = reinterpret_cast<const unsigned short*>(a.X + (long long)(tok0 + r) * a.ldx + k);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) w[c] = u[2 * c] | ((uint32_t)u[2 * c + 1] << 16);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(su32(ringB) + slot * slot_bytes +
+                                                                          (pc >> 3) * half_bytes + r * 128 +
+                                                                          (((pc ^ r) & 7) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (kSums)
+          for (int r = 32 * aw; r < 32 * aw + 32 && r < p.N; r += 16) sums(j, r);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mb_arrive(&full[slot]);
+      }
+  } else if (warp < 16) {
+    // the words of this thread's row: 8 bytes of each 16 of its pair of rows' 64 in
+    // every chunk of its tile, conflict-free
+    const int dg = (warp - 8) >> 2, g = lane & 7, hi = (lane >> 3) & 1, row = quad * 32 + lane;  // dg: even or odd steps
+    const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16) + kAcc * 64;
+    const uint32_t zp2 = (0x4180u + ((AWQ ? (uint32_t)a.zp : 8u) << 3)) * 0x10001u;  // 16 + zp, zp < 16
+    uint32_t woff[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) woff[t] = (2 * quad + (lane >> 4)) * kBB + (g * 4 + (t ^ (g >> 1))) * 16 + hi * 8;
+    if (dg == 1 && (j0 & 1)) {  // the first block holds no step of this group
+      ok = warp_wait(&wFull[0], 0);
+      if (lane == 0) mb_arrive(&wEmpty[0]);
+    }
     for (int j = dg; j < n && ok; j += 2) {
-      if (j >= kASlots) {  // the slot's last MMAs
+      const int bi = ((j0 + j) >> 1) - b0, slot = bi % kRing, odd = (j0 + j) & 1;
+      if (j >= kASlots) {  // the A slot's last MMAs
         const int o = j - kASlots;
-        if (!warp_wait(&empty[o & 3], (o >> 2) & 1)) {
+        if (!warp_wait(&empty[o % kXSlots], o / kXSlots & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
       }
-      const uint32_t ta = tl + (j % kASlots) * (256 / kASlots);
+      if (!warp_wait(&wFull[slot], (bi / kRing) & 1)) {
+        ok = false;
+        break;
+      }
+      const unsigned char* wb = ringW + slot * 8 * kBB;
+      const uint32_t ta = tl + j % kASlots * C::kACols;
       uint32_t shi[kGs], slo[kGs];  // the groups' scales as pairs of two bf16 terms
       if (kSplit) {
+        uint32_t zw[16];  // three bf16 terms of z + 8 s against three of the sum: six columns a group
 #pragma unroll
-        for (int q = 0; q < kGs; ++q) {
-          const float f = __half2float(__ushort_as_half(sraw[q]));
-          shi[q] = bf2_dup(f);
-          slo[q] = bf2_dup(f - __uint_as_float(shi[q] << 16));
+        for (int c = 0; c < 16; ++c) zw[c] = 0;
+#pragma unroll
+        for (int c = 0; c < kGs; ++c) {
+          const unsigned char* sp = wb + (row >> 4) * kBB + 2048 + (odd * kGs + c) * 32 + g * 4 + hi * 2;
+          const float f = __half2float(*reinterpret_cast<const __half*>(sp));
+          shi[c] = bf2_dup(f);
+          slo[c] = bf2_dup(f - __uint_as_float(shi[c] << 16));
+          if (kZCols) {
+            const Terms m = bf16_terms(fmaf(8.f, f, __half2float(*reinterpret_cast<const __half*>(sp + kGrp * 32))));
+            zw[3 * c] = bf2_pack(m.v0, m.v0), zw[3 * c + 1] = bf2_pack(m.v0, m.v1), zw[3 * c + 2] = bf2_pack(m.v1, m.v2);
+          }
         }
-        if (j + 2 < n) fetch_scales(j0 + j + 2);
+        if (kZCols) {
+          const uint32_t zp = su32(ringZ) + j % kASlots * 16384 + row * 128;
+#pragma unroll
+          for (int c = 0; c < kGs; ++c)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(zp + ((c ^ (row & 7)) << 4)), "r"(zw[4 * c]),
+                         "r"(zw[4 * c + 1]), "r"(zw[4 * c + 2]), "r"(zw[4 * c + 3])
+                         : "memory");
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        uint2 raw[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) raw[t] = *reinterpret_cast<const uint2*>(wb + (odd * 2 + h) * 512 + woff[t]);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
           uint32_t r[16], lo[16];
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
+            const uint32_t w = kb ? raw[t].y : raw[t].x;  // k = 32 kb + 8 t + {0..7}
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {  // word (kb, kt): k = 32 kb + 8 t + 4 kt + {0..3}
-              const uint4& u = raw[h][t];
-              const uint32_t w = kb ? (kt ? u.w : u.z) : (kt ? u.y : u.x);
-              const uint32_t v = __funnelshift_r(w, w, rot);
-              const int col = 4 * t + 2 * kt;
-              r[col] = nib16(v);
-              r[col + 1] = nib16(__funnelshift_r(v, v, 8));
-              r[col] = bf2_sub(r[col], zp2);
-              r[col + 1] = bf2_sub(r[col + 1], zp2);
-            }
+            for (int c = 0; c < 4; ++c) r[4 * t + c] = bf2_sub(nib16(__funnelshift_r(w, w, 4 * c)), zp2);
           }
           if (kSplit) {
-            const uint32_t hi = shi[kGs == 4 ? 2 * h + kb : h], sl = slo[kGs == 4 ? 2 * h + kb : h];
+            const uint32_t sh = shi[kGs == 4 ? 2 * h + kb : h], sl = slo[kGs == 4 ? 2 * h + kb : h];
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               const uint32_t q = r[c];
-              r[c] = bf2_mul(q, hi);
-              lo[c] = bf2_fma(q, sl, bf2_fma(q, hi, r[c] ^ 0x80008000u));
+              r[c] = bf2_mul(q, sh);
+              lo[c] = bf2_fma(q, sl, bf2_fms(q, sh, r[c]));
             }
             tmem_st16(ta + 64 + 32 * h + 16 * kb, lo);
           }
           tmem_st16(ta + 32 * h + 16 * kb, r);
         }
-        if (j + 2 < n) fetch(h, j0 + j + 2);
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      if (kZCols) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mb_arrive(&full[j & 3]);
+      if (lane == 0) {
+        mb_arrive(&full[j % kXSlots]);
+        mb_arrive(&wEmpty[slot]);
+      }
     }
   } else if (ncol > 0) {
     const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16) + cbeg;
     const int row = quad * 32 + lane;
-    float acc[32];
+    uint64_t acc[16];  // pairs of columns
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    // The columns come in two halves of 16; a half's load is in flight while the
-    // one before it is added, across steps.
-    uint32_t lo[16], up[16];
-    ok = warp_wait(&accFull[0], 0);
-    tc_fence_after();
-    if (ok) tmem_ld16_issue(tq, lo);
-    for (int j = 0; ok && j < n; ++j) {
-      const int side = j & (kUSide - 1), buf = j & 3;
-      // pair (g, g + 8) of the row's tile in the step's first scale group
-      const int si = (side * 8 + (row >> 4)) * kGs * 16 + (row & 7) * 2 + ((row >> 3) & 1);
-      const float s = kSplit ? 1.f : __half2float(sc[si]);
-      const float* x = xs + side * kGs * kUCols + cbeg;
-      auto add = [&](const uint32_t (&v)[16], int c0) {
+    for (int i = 0; i < 16; ++i) acc[i] = 0;
+    uint32_t phase = 0;  // bit w: parity of accumulator w's next drain
+    // cols: this warp's columns, as a constant
+    auto drain = [&](auto cols) {
+      constexpr int kC = decltype(cols)::value;
+      for (int j = 0; j < n; ++j) {
+        if (!drained(j)) continue;
+        const int buf = j % kAcc;
+        if (!warp_wait(&accFull[buf], (phase >> buf) & 1)) {
+          ok = false;
+          break;
+        }
+        phase ^= 1u << buf;
+        tc_fence_after();
+        float v[kC];
+        tmem_ld<kC>(tq + buf * 64, v);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mb_arrive(&accEmpty[buf]);
+        if (kSplit) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          acc[c0 + c] = kSplit ? acc[c0 + c] + __uint_as_float(v[c]) : fmaf(s, __uint_as_float(v[c]), acc[c0 + c]);
-        if (kSums)
+          for (int c = 0; c < kC; c += 2) acc[c >> 1] = f2_add(acc[c >> 1], f2_pack(v[c], v[c + 1]));
+        } else {
+          const int bi = ((j0 + j) >> 1) - b0, slot = bi % kRing, odd = (j0 + j) & 1;
+          if (!warp_wait(&wFull[slot], (bi / kRing) & 1)) {
+            ok = false;
+            break;
+          }
+          // pair (g, g + 8) of the row's tile
+          const unsigned char* sp =
+              ringW + (slot * 8 + (row >> 4)) * kBB + 2048 + odd * 32 + (row & 7) * 4 + ((row >> 3) & 1) * 2;
+          const float f = __half2float(*reinterpret_cast<const __half*>(sp));
+          const float zf = kSums ? fmaf(8.f, f, __half2float(*reinterpret_cast<const __half*>(sp + kGrp * 32))) : 0.f;
+          if (odd || j == n - 1) {
+            __syncwarp();
+            if (lane == 0) mb_arrive(&wEmpty[slot]);
+          }
+          const uint64_t s = f2_pack(f, f);
 #pragma unroll
-          for (int q = 0; q < kGs; ++q) {
-            const int sq = si + q * 16;
-            const float z = fmaf(8.f, __half2float(sc[sq]), __half2float(zr[sq]));
+          for (int c = 0; c < kC; c += 2) acc[c >> 1] = f2_fma(s, f2_pack(v[c], v[c + 1]), acc[c >> 1]);
+          if (kSums) {
+            const uint64_t z = f2_pack(zf, zf);
+            const float* x = xs + (j & (kUSide - 1)) * kUCols + cbeg;
 #pragma unroll
-            for (int c = 0; c < 16; c += 4) {
-              const float4 xv = *reinterpret_cast<const float4*>(x + q * kUCols + c0 + c);
-              acc[c0 + c] = fmaf(z, xv.x, acc[c0 + c]), acc[c0 + c + 1] = fmaf(z, xv.y, acc[c0 + c + 1]);
-              acc[c0 + c + 2] = fmaf(z, xv.z, acc[c0 + c + 2]), acc[c0 + c + 3] = fmaf(z, xv.w, acc[c0 + c + 3]);
+            for (int c = 0; c < kC; c += 4) {
+              const float4 xv = *reinterpret_cast<const float4*>(x + c);
+              acc[c >> 1] = f2_fma(z, f2_pack(xv.x, xv.y), acc[c >> 1]);
+              acc[(c >> 1) + 1] = f2_fma(z, f2_pack(xv.z, xv.w), acc[(c >> 1) + 1]);
             }
           }
-      };
-      tmem_ld16_wait(lo);
-      if (ncol > 16) {
-        tmem_ld16_issue(tq + buf * 64 + 16, up);
-        add(lo, 0);
-        tmem_ld16_wait(up);
+        }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mb_arrive(&accEmpty[buf]);
-      if (ncol <= 16) {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) up[c] = lo[c];
-      }
-      if (j + 1 < n) {
-        const int nb = (j + 1) & 3;
-        ok = warp_wait(&accFull[nb], ((j + 1) >> 2) & 1);
-        tc_fence_after();
-        if (ok) tmem_ld16_issue(tq + nb * 64, lo);
-      }
-      if (ncol > 16)
-        add(up, 16);
-      else
-        add(up, 0);
-    }
+    };
+    if (ncol > 16)
+      drain(std::integral_constant<int, 32>{});
+    else
+      drain(std::integral_constant<int, 16>{});
     // this warp has seen every MMA of the CTA complete: the B slots are free
-    if (p.c > 1) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (c < ncol) red[(cbeg + c) * 128 + row] = acc[c];
-    } else {
-      const int m = unit * 128 + row, left = m < a.M ? min(ncol, a.T - tok0 - cbeg) : 0;
-      if (a.R) {
-        const __nv_bfloat16* r = a.R + (long long)(tok0 + cbeg) * a.ldr + m;
-#pragma unroll
-        for (int c = 0; c < 32; ++c, r += a.ldr)
-          if (c < left) acc[c] += __bfloat162float(*r);
+    for (int c = 0; c < 16; ++c)
+      if (2 * c < ncol) {
+        const float2 v = f2_unpack(acc[c]);
+        red[(cbeg + 2 * c) * 128 + row] = v.x;
+        red[(cbeg + 2 * c + 1) * 128 + row] = v.y;
       }
-      if (a.y_f32) {
-        float* y = reinterpret_cast<float*>(a.Y) + (long long)(tok0 + cbeg) * a.ldy + m;
-#pragma unroll
-        for (int c = 0; c < 32; ++c, y += a.ldy)
-          if (c < left) *y = acc[c];
-      } else {
-        __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(a.Y) + (long long)(tok0 + cbeg) * a.ldy + m;
-#pragma unroll
-        for (int c = 0; c < 32; ++c, y += a.ldy)
-          if (c < left) *y = __float2bfloat16_rn(acc[c]);
-      }
-    }
   }
   if (!ok && a.err) atomicOr(a.err, 1);
   tc_fence_before();
@@ -474,22 +621,33 @@ __global__ void __launch_bounds__(kULinThreads, 1) k_lin_umma(const LinArgs a, c
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
-  if (p.c == 1) return;
-  u_cluster_sync();
+  if (p.c > 1) u_cluster_sync();
   const uint32_t local = su32(red);
   const int cols = min(p.N, a.T - tok0);
+#pragma unroll 2
   for (int e = threadIdx.x + rank * kULinThreads; e < cols * 128; e += kULinThreads * p.c) {
     float v = 0.f;
-    for (int q = 0; q < p.c; ++q) {
-      uint32_t at;
-      float w;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local + e * 4), "r"(q));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(at) : "memory");
-      v += w;
+    if (p.c == 1) {
+      v = red[e];
+    } else {
+      for (int q = 0; q < p.c; ++q) {
+        uint32_t at;
+        float w;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local + e * 4), "r"(q));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(at) : "memory");
+        v += w;
+      }
     }
-    store(unit * 128 + (e & 127), tok0 + (e >> 7), v);
+    const int row = unit * 128 + (e & 127);
+    const long long tok = tok0 + (e >> 7);
+    if (row >= a.M) continue;
+    if (a.R) v += __bfloat162float(a.R[tok * a.ldr + row]);
+    if (a.y_f32)
+      reinterpret_cast<float*>(a.Y)[tok * a.ldy + row] = v;
+    else
+      reinterpret_cast<__nv_bfloat16*>(a.Y)[tok * a.ldy + row] = __float2bfloat16_rn(v);
   }
-  u_cluster_sync();  // no CTA leaves while another reads its partial sums
+  if (p.c > 1) u_cluster_sync();  // no CTA leaves while another reads its partial sums
 }
 
 template <int FL, bool AWQ>
@@ -507,10 +665,10 @@ cudaError_t launch_u(const LinArgs& a, cudaStream_t st) {
     const long long now = (units * c + resident[c] - 1) / resident[c] * ((p.steps + c - 1) / c + 10);
     if (cost < 0 || now < cost) cost = now, p.c = c;
   }
-  constexpr int side = kUSide * (4 / FL) * (kUCols * 4 + 128 * 2 * (AWQ ? 1 : 2));
-  const int smem = kUSteps * p.N * 256 + side + 1024;
-  constexpr int most = kUSteps * kUCols * 256 + side + 1024;
-  static_assert(most <= 227 * 1024, "shared memory");
+  const int smem = UCfg<FL, AWQ>::smem(p.N);
+  constexpr int most = UCfg<FL, AWQ>::smem(kUCols);
+  CUtensorMap xmap{};
+  p.tma = a.x_vec && b_tensor_map(&xmap, a.X, a.K, a.T, a.ldx, p.N);
   const auto kernel = k_lin_umma<FL, AWQ>;
   static bool attr[64] = {false};
   int dev = 0;
@@ -535,7 +693,7 @@ cudaError_t launch_u(const LinArgs& a, cudaStream_t st) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.c > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a, p);
+  return cudaLaunchKernelEx(&cfg, kernel, a, p, xmap);
 }
 
 }  // namespace

@@ -32,6 +32,17 @@ __device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t par) {
       : "memory");
   return ok != 0;
 }
+// As mb_try, but returns at once (try_wait may suspend the thread for a while).
+__device__ __forceinline__ bool mb_test(uint64_t* b, uint32_t par) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(su32(b)), "r"(par)
+      : "memory");
+  return ok != 0;
+}
 // As mb_try, but a waiting thread is suspended (not spinning, so it takes no
 // issue slots from the working warps) until the phase completes or about
 // kSuspendNs have passed.
@@ -108,6 +119,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(su32(bar))
       : "memory");
 }
+
+// Host (int4_umma.cu): the map of `rows` x K bf16 rows, ld elements apart, for
+// tma_load_2d; false when they cannot be read that way (alignment, strides).
+bool b_tensor_map(CUtensorMap* m, const void* base, int K, int rows, long long ld, int box_rows);
 
 // Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups
 // 1024 bytes apart (SBO), Blackwell descriptor version 1.
