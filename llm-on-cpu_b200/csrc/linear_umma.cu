@@ -18,7 +18,7 @@
 //     a product like the others, in six more columns of A and B per group: z + 8 s
 //     and xs, three bf16 terms (24 bits) each, the six largest of their products.
 //     A drain per group of 32 instead took 51 us at T = 37, 4101 x 7264 with zeros,
-//     and the zeros added in the drain 28.7 us, against 26.
+//     and the zeros added in the drain 28.7 us, against 18.1.
 //     Two steps per drain, not four: the tensor core's sums are truncated, and
 //     four steps' err by 8e-7 of the output's norm at K = 16384, two steps' by 6e-7.
 //
@@ -33,13 +33,15 @@
 //                 costs its issuing thread 75 to 100 cycles); small groups: two warps
 //   warp  4       activations by TMA (unaligned ones: warps 6, 7 with plain loads)
 //   warp  5       weights: a bulk copy per tile and block of two steps, blocks ahead
-//   warps 6, 7    GPTQ: the group sums of what landed (mma.sync with ones)
+//   warps 6, 7    GPTQ: the group sums of what landed (mma.sync with ones and zeros)
 //   warps 8..15   dequantisers, thread = weight row = TMEM lane, even and odd steps
 //   warps 16..23  drain, one lane quadrant and half of the columns each
 //
 // Loads through registers or cp.async were the bound before: an SM got 15 bytes per
-// clock of activations that all CTAs read (T = 64, 11008 x 4096: 22.8 us, now 20.1;
-// groups of 32: 42.4, now 27.8).
+// clock of activations that all CTAs read (T = 64, 11008 x 4096: 22.8 us, now 19.2;
+// groups of 32: 42.4, now 26.0).  Now it is the instructions of 24 warps, of which a
+// step of 128 k costs 0.45 us, 0.6 with small groups; groups of 128 wait for the
+// drain, small groups for the dequantisers and, with zeros, the sums.
 //
 // K splits over the CTAs of a cluster; their partial sums meet in distributed
 // shared memory and are added in rank order.  Every wait is bounded; one that
@@ -153,12 +155,11 @@ __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-// d[0], d[1] += the sums over 16 k of tokens 2 t, 2 t + 1 (every row the same)
-__device__ __forceinline__ void mma_ones(float (&d)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, {%0,%1,%2,%3};"
+// d += a b of m16n8k16
+__device__ __forceinline__ void mma_sum(float (&d)[4], const uint32_t (&a)[4], uint32_t b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%8}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(0x3F803F80u), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b));
 }
 __device__ __forceinline__ void u_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -370,48 +371,46 @@ __global__ void __launch_bounds__(kULinThreads, 1)
   } else if (warp < 8) {
     // activations of 32 tokens: loaded here where TMA cannot, and their group sums
     const int aw = warp - 6, g = lane >> 2, t = lane & 3, pc = lane & 15;
-    // The sums come from mma.sync with a row of ones, 32 k of 8 tokens per pair;
-    // every lane of a column gets them, and lane (g, t) writes those of scale group q
-    // for token 2 t + e
-    const int q = g % kGs, e = (g / kGs) & 1;
-    auto sums = [&](int j, int row0) {  // 16 tokens from row0
+    // The sums come from mma.sync: 16 tokens times a B that is one in the columns of
+    // the group at hand, so that lane (g, t) ends with tokens g and g + 8 of group q
+    constexpr int kDup = 4 / kGs;  // lanes with the same sums: they write in turn
+    const int q = t / kDup;
+    const int row0[2] = {32 * aw, 32 * aw + (32 * aw + 16 < p.N ? 16 : 0)};  // twice 16 tokens, or the same ones
+    auto sums = [&](int j) {
       const uint32_t slot = su32(ringB) + j % kXSlots * slot_bytes;
-      const int trow = row0 + 2 * t + e;
-      float v[2][kGs][2];
+      float d[2][4] = {};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t rows = slot + (row0 + 8 * i + (lane & 7)) * 128;
-        float d[4];
+      for (int h = 0; h < 2; ++h) {  // 64 k: 16-byte pieces 2 k, 2 k + 1
+        uint32_t x[2][4][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // 32 k: 16-byte pieces 4 k .. 4 k + 3
-          uint32_t b[4];
-          ldmatrix4(rows + (k >> 1) * half_bytes + ((((k & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b);
-          if (k % FL == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
-          mma_ones(d, b[0], b[1]);
-          mma_ones(d, b[2], b[3]);
-          if (k % FL == FL - 1) v[i][k / FL][0] = d[0], v[i][k / FL][1] = d[1];
-        }
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            ldmatrix4(slot + (row0[r] + (lane & 15)) * 128 + h * half_bytes + (((2 * k + (lane >> 4)) ^ (lane & 7)) << 4),
+                      x[r][k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) mma_sum(d[r], x[r][k], (4 * h + k) / (2 * FL) == g / (2 * kDup) ? 0x3F803F80u : 0u);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (kGs < 4 && (g / (2 * kGs)) % 2 != i) continue;  // fewer groups: a lane writes for one of the two
-        float x = v[i][0][0];
-#pragma unroll
-        for (int c = 1; c < 2 * kGs; ++c)
-          if (c == q + e * kGs) x = v[i][c % kGs][c / kGs];
+      for (int c = 0; c < 4; ++c) {
+        if (kDup > 1 && (t & 1) != (c & 1)) continue;
+        const float x = d[c >> 1][2 * (c & 1)];
+        const int row = row0[c >> 1] + g + 8 * (c & 1);
         if (kZCols) {
           const Terms m = bf16_terms(x);
           const uint32_t w[3] = {bf2_pack(m.v0, m.v1), bf2_pack(m.v2, m.v0), bf2_pack(m.v1, m.v0)};
 #pragma unroll
           for (int c = 0; c < 3; ++c) {
             const int wi = 3 * q + c;
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + 2 * half_bytes + (trow + 8 * i) * 128 +
-                                                         (((wi >> 2) ^ (trow & 7)) << 4) + (wi & 3) * 4),
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + 2 * half_bytes + row * 128 +
+                                                         (((wi >> 2) ^ (row & 7)) << 4) + (wi & 3) * 4),
                          "r"(w[c])
                          : "memory");
           }
         } else {
-          xs[(j & (kUSide - 1)) * kUCols + trow + 8 * i] = x;
+          xs[(j & (kUSide - 1)) * kUCols + row] = x;
         }
       }
     };
@@ -447,8 +446,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
         }
         if (!ok) break;
         __syncwarp();
-        if (kSums)
-          for (int r = 32 * aw; r < 32 * aw + 32 && r < p.N; r += 16) sums(j, r);
+        if (kSums && 32 * aw < p.N) sums(j);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mb_arrive(&full[slot]);
@@ -549,6 +547,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
     uint64_t acc[16];  // pairs of columns
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0;
+    int slot = 0, wpar = 0;  // the weight block's place and parity
     uint32_t phase = 0;  // bit w: parity of accumulator w's next drain
     // cols: this warp's columns, as a constant
     auto drain = [&](auto cols) {
@@ -556,6 +555,24 @@ __global__ void __launch_bounds__(kULinThreads, 1)
       for (int j = 0; j < n; ++j) {
         if (!drained(j)) continue;
         const int buf = j % kAcc;
+        float f = 1.f, zf = 0.f;  // the row's scale, and z + 8 s
+        if (!kSplit) {
+          const int odd = (j0 + j) & 1;
+          if (!(odd && j) && !warp_wait(&wFull[slot], wpar)) {  // once a block
+            ok = false;
+            break;
+          }
+          // pair (g, g + 8) of the row's tile
+          const unsigned char* sp =
+              ringW + (slot * 8 + (row >> 4)) * kBB + 2048 + odd * 32 + (row & 7) * 4 + ((row >> 3) & 1) * 2;
+          f = __half2float(*reinterpret_cast<const __half*>(sp));
+          if (kSums) zf = fmaf(8.f, f, __half2float(*reinterpret_cast<const __half*>(sp + kGrp * 32)));
+          if (odd || j == n - 1) {
+            __syncwarp();
+            if (lane == 0) mb_arrive(&wEmpty[slot]);
+            if (++slot == kRing) slot = 0, wpar ^= 1;
+          }
+        }
         if (!warp_wait(&accFull[buf], (phase >> buf) & 1)) {
           ok = false;
           break;
@@ -571,20 +588,6 @@ __global__ void __launch_bounds__(kULinThreads, 1)
 #pragma unroll
           for (int c = 0; c < kC; c += 2) acc[c >> 1] = f2_add(acc[c >> 1], f2_pack(v[c], v[c + 1]));
         } else {
-          const int bi = ((j0 + j) >> 1) - b0, slot = bi % kRing, odd = (j0 + j) & 1;
-          if (!warp_wait(&wFull[slot], (bi / kRing) & 1)) {
-            ok = false;
-            break;
-          }
-          // pair (g, g + 8) of the row's tile
-          const unsigned char* sp =
-              ringW + (slot * 8 + (row >> 4)) * kBB + 2048 + odd * 32 + (row & 7) * 4 + ((row >> 3) & 1) * 2;
-          const float f = __half2float(*reinterpret_cast<const __half*>(sp));
-          const float zf = kSums ? fmaf(8.f, f, __half2float(*reinterpret_cast<const __half*>(sp + kGrp * 32))) : 0.f;
-          if (odd || j == n - 1) {
-            __syncwarp();
-            if (lane == 0) mb_arrive(&wEmpty[slot]);
-          }
           const uint64_t s = f2_pack(f, f);
 #pragma unroll
           for (int c = 0; c < kC; c += 2) acc[c >> 1] = f2_fma(s, f2_pack(v[c], v[c + 1]), acc[c >> 1]);
@@ -623,29 +626,53 @@ __global__ void __launch_bounds__(kULinThreads, 1)
   }
   if (p.c > 1) u_cluster_sync();
   const uint32_t local = su32(red);
-  const int cols = min(p.N, a.T - tok0);
-#pragma unroll 2
-  for (int e = threadIdx.x + rank * kULinThreads; e < cols * 128; e += kULinThreads * p.c) {
-    float v = 0.f;
-    if (p.c == 1) {
-      v = red[e];
-    } else {
-      for (int q = 0; q < p.c; ++q) {
-        uint32_t at;
-        float w;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local + e * 4), "r"(q));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(at) : "memory");
-        v += w;
+  // a thread stores two rows for every 12 c-th token
+  constexpr int per = kULinThreads / 64;
+  const int cols = min(p.N, a.T - tok0), row = 2 * (threadIdx.x & 63), m = unit * 128 + row;
+  int col = (threadIdx.x >> 6) + rank * per;
+  if (m < a.M && col < cols) {
+    const bool two = m + 1 < a.M;
+    const int es = a.y_f32 ? 4 : 2;
+    char* y = reinterpret_cast<char*>(a.Y) + ((long long)(tok0 + col) * a.ldy + m) * es;
+    const __nv_bfloat16* r = a.R + (a.R ? (long long)(tok0 + col) * a.ldr + m : 0);
+#pragma unroll 1
+    for (; col < cols; col += per * p.c, y += per * p.c * a.ldy * es, r += per * p.c * a.ldr) {
+      float2 v = make_float2(0.f, 0.f);
+      if (a.R) {
+        v.x = __bfloat162float(r[0]);
+        if (two) v.y = __bfloat162float(r[1]);
+      }
+      float2 s = make_float2(0.f, 0.f);
+      if (p.c == 1) {
+        s = *reinterpret_cast<const float2*>(red + col * 128 + row);
+      } else {
+        float2 w[8];  // the ranks' parts, all on their way at once
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          w[q] = make_float2(0.f, 0.f);
+          if (q < p.c) {
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local + (col * 128 + row) * 4), "r"(q));
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(w[q].x), "=f"(w[q].y) : "r"(at) : "memory");
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s.x += w[q].x, s.y += w[q].y;
+      }
+      v.x += s.x, v.y += s.y;
+      if (a.y_vec && two) {
+        if (a.y_f32)
+          *reinterpret_cast<float2*>(y) = v;
+        else
+          *reinterpret_cast<__nv_bfloat162*>(y) = __float22bfloat162_rn(v);
+      } else if (a.y_f32) {
+        reinterpret_cast<float*>(y)[0] = v.x;
+        if (two) reinterpret_cast<float*>(y)[1] = v.y;
+      } else {
+        reinterpret_cast<__nv_bfloat16*>(y)[0] = __float2bfloat16_rn(v.x);
+        if (two) reinterpret_cast<__nv_bfloat16*>(y)[1] = __float2bfloat16_rn(v.y);
       }
     }
-    const int row = unit * 128 + (e & 127);
-    const long long tok = tok0 + (e >> 7);
-    if (row >= a.M) continue;
-    if (a.R) v += __bfloat162float(a.R[tok * a.ldr + row]);
-    if (a.y_f32)
-      reinterpret_cast<float*>(a.Y)[tok * a.ldy + row] = v;
-    else
-      reinterpret_cast<__nv_bfloat16*>(a.Y)[tok * a.ldy + row] = __float2bfloat16_rn(v);
   }
   if (p.c > 1) u_cluster_sync();  // no CTA leaves while another reads its partial sums
 }

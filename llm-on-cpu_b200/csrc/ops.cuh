@@ -29,6 +29,7 @@ struct LinArgs {
   long long ldy;
   int y_f32;
   int x_vec;  // X rows readable by 16-byte loads
+  int y_vec;  // two neighbours of Y, the first in an even column, writable at once
   int* err;   // bit 0: a bounded wait gave up
 };
 struct LinPack {

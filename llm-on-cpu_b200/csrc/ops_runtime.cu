@@ -270,6 +270,7 @@ llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* L, const uint16_
   a.ldy = ldy;
   a.y_f32 = y_dtype == LLMOC_DTYPE_F32;
   a.x_vec = aligned(X, 16) && ldx % 8 == 0;
+  a.y_vec = aligned(Y, a.y_f32 ? 8 : 4) && ldy % 2 == 0;
   a.err = L->err;
   return launched(launch_linear(a, L->fl, L->awq, (cudaStream_t)stream), who, 1);
 }
