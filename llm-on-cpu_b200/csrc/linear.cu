@@ -13,16 +13,25 @@
 // (g, g + 8).  Groups that are other multiples of 32, 64 or 128 repeat their
 // scale, so a block holds 8, 4 or 2 groups of 32, 64 or 128.
 //
-// Work.  A warp owns RT tiles against NT * 8 tokens over a slice of K.  The
-// eight warps of a CTA take 8 / ksw tile groups and split K ksw ways; a cluster
+// Work.  A warp owns a tile against NT * 8 tokens over a slice of K.  The
+// 16 warps of a CTA take 16 / ksw tiles and split K ksw ways; a cluster
 // of c CTAs splits K c ways more.  With c = ksw = 1 a CTA walks tile groups
 // (persistent) and its warps never meet; otherwise the partial sums meet in
 // (distributed) shared memory and are added in slice order, so no workspace is
 // needed and the bits do not depend on timing.
 //
-// The stream runs through a ring of registers, 4 KB per warp: a chunk is one
-// coalesced 16-byte load per lane, reissued for the place 8 / RT chunks further
-// on as soon as it is consumed, across tile ends.
+// The stream runs through a ring in shared memory per warp, filled by one bulk
+// copy per block and tile as soon as a place has been read, across tile ends, so
+// up to 8 blocks (17 to 20 KB) of a warp are on their way.  Loads into a ring of
+// registers brought 15 to 18 bytes per clock and SM at most and took the issue
+// slots that dequantisation needs (248320 x 2048, T = 8: 57.1 us, now 55.0; groups
+// of 32: 77.8, now 61.6; 11008 x 4096, T = 8: 16.0, now 12.4).  One CTA per SM, so
+// that the activations are staged once.
+//
+// What bounds it now: with T = 1 at 248320 x 2048 52.5 us are 4.97 TB/s; with the
+// shifts of the dequantisation left out (and wrong results) the same kernel takes
+// 41.5 us, the rate of a plain copy.  Three of four register pairs need one, they
+// run at half rate, and a product by a power of two in their place is slower.
 //
 // Dequantisation.  A word holds eight nibbles, pair j of them (one per 16-bit
 // half) at bits 3 + 4j: rotated right by 4j and merged into 0x4180 it is the
@@ -41,27 +50,17 @@
 #include <string>
 
 #include "ops.cuh"
+#include "umma_dev.cuh"
 
 namespace llmoc {
 
 namespace {
 
-constexpr int kLinWarps = 8;
+constexpr int kLinWarps = 16, kLinWarpsLog = 4;
 constexpr int kLinThreads = kLinWarps * 32;
+constexpr int kRingMax = 8;      // places of a warp's ring at most
 constexpr uint32_t kOffset = 16;  // A elements are kOffset + q
 
-__device__ __forceinline__ uint4 ld_stream(const char* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t ld_pair(const char* p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ float2 pair_f32(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 __device__ __forceinline__ uint32_t nib_pair(uint32_t w) {  // (16 + q_lo, 16 + q_hi) as bf16
   uint32_t d;
@@ -93,25 +92,28 @@ __device__ __forceinline__ float ld_cluster(const float* p, int rank, int c) {
 struct LinPlan {
   int lk;     // log2 of ksw, the warps of a CTA that split K
   int lc;     // log2 of c, the CTAs of a cluster that split K
-  int units;  // tile groups (8 / ksw warps x RT tiles)
+  int units;  // tile groups (of 16 / ksw tiles)
   int bps;    // blocks of 256 k per staged slab
   int nslab;  // slabs of a CTA's share of K
+  int ring;   // places of a warp's ring, each a block of its tile
 };
 
 // FL: 32-wide blocks per scale group (1, 2, 4); TP: token rows staged (1, or
 // NT * 8).
-template <int FL, bool AWQ, int NT, int RT, int TP>
-__global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, const LinPlan p) {
+template <int FL, bool AWQ, int NT, int TP>
+__global__ void __launch_bounds__(kLinThreads, 1) k_linear(const LinArgs a, const LinPlan p) {
   constexpr int kBB = lin_block_bytes(FL, !AWQ);
-  constexpr int GB = 2 / RT;                    // blocks in flight per tile
   constexpr int kGrp = 8 / FL;                  // scale groups per block
-  constexpr int kRows = RT * 16, kCols = NT * 8, kColLd = kRows + 4;
+  constexpr int kCols = NT * 8, kColLd = 16 + 4;
   constexpr int kXW = TP * 4;                   // 16-byte pieces per 32 k
-  extern __shared__ __align__(16) uint4 sx[];   // [slab's 32-blocks][kXW]: B fragments
+  extern __shared__ __align__(128) char lsm[];  // [warp][ring][kBB]: the weights as they are stored
+  __shared__ __align__(8) uint64_t landed[kLinWarps][kRingMax];
+  __shared__ volatile int abort_flag;
+  uint4* sx = reinterpret_cast<uint4*>(lsm + kLinWarps * p.ring * kBB);  // [slab's 32-blocks][kXW]: B fragments
   float* xs = reinterpret_cast<float*>(sx + (size_t)p.bps * 8 * kXW);  // [slab's groups][TP]: activation sums
   float* red = xs + (size_t)p.bps * kGrp * TP;                         // [warp][col][row]: partial sums
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int c = 1 << p.lc, ksw = 1 << p.lk, lr = 3 - p.lk;  // lr: log2 of the CTA's tile groups
+  const int c = 1 << p.lc, ksw = 1 << p.lk, lr = kLinWarpsLog - p.lk;  // lr: log2 of the CTA's tile groups
   const int rank = blockIdx.x & (c - 1), ncl = gridDim.x >> p.lc;
   const int tok0 = blockIdx.y * kCols;
   const int wt = warp & ((1 << lr) - 1), wk = warp >> lr;
@@ -128,49 +130,57 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
   auto seg_of = [&](int unit, int slab) {
     Seg s;
     const int s0 = p0 + slab * p.bps, n = max(0, min(p1, s0 + p.bps) - s0);
-    const int tile = ((unit << lr) + wt) * RT;
+    const int tile = (unit << lr) + wt;
     s.b0 = n * wk >> p.lk;
     s.nb = tile < a.mt && unit < p.units ? (n * (wk + 1) >> p.lk) - s.b0 : 0;
     s.q = a.q + (size_t)min(tile, a.mt - 1) * tile_bytes + (size_t)(s0 + s.b0) * kBB;
     return s;
   };
-  uint4 qw[GB][4][RT];
-  uint32_t sw[GB][kGrp][RT], zw[GB][kGrp][RT];
-  // a tile past the end reads the last one again; its rows are not stored
-  auto tile_off = [&](int r, int unit) { return r && ((unit << lr) + wt) * RT + r < a.mt ? tile_bytes : 0; };
   const int lq = (g * 4 + (t ^ ((g >> 1) & 3))) * 16, ls = 2048 + g * 4;
+  char* ring = lsm + warp * p.ring * kBB;
+  uint64_t* bar = landed[warp];
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < p.ring; ++i) mb_init(&bar[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  // the next block to fetch: the segments in the order of use
+  int iunit = blockIdx.x >> p.lc, islab = 0, ib = 0, islot = 0;
+  uint32_t issued = 0;
+  bool bad = false;
+  Seg is = seg_of(iunit, 0);
+  auto fetch = [&]() {  // into the next place, which is free
+    while (iunit < p.units && ib >= is.nb) {
+      if (++islab == p.nslab) islab = 0, iunit += ncl;
+      is = seg_of(iunit, islab), ib = 0;
+    }
+    if (iunit >= p.units || bad) return;
+    if (lane == 0) {
+      mb_expect(&bar[islot], kBB);
+      bulk_g2s(su32(ring + islot * kBB), is.q + (size_t)ib * kBB, kBB, &bar[islot]);
+    }
+    ++ib, ++issued;
+    if (++islot == p.ring) islot = 0;
+  };
+  for (int i = 0; i < p.ring; ++i) fetch();  // the weights do not depend on the previous kernel
+  int slot = 0, par = 0;
 
   int unit = blockIdx.x >> p.lc, slab = 0;
   Seg cur = seg_of(unit, 0);
-#pragma unroll
-  for (int j = 0; j < GB; ++j)  // the weights do not depend on the previous kernel
-    if (j < cur.nb)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const char* q = cur.q + tile_off(r, unit) + j * kBB;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qw[j][i][r] = ld_stream(q + lq + i * 512);
-#pragma unroll
-        for (int i = 0; i < kGrp; ++i) {
-          sw[j][i][r] = ld_pair(q + ls + i * 32);
-          if (!AWQ) zw[j][i][r] = ld_pair(q + ls + (kGrp + i) * 32);
-        }
-      }
   grid_dep_wait();
   grid_dep_release();
 
-  float acc[RT][NT][4], part[RT][NT][4];
+  float acc[NT][4], part[NT][4];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[r][n][i] = part[r][n][i] = 0.f;
+    for (int i = 0; i < 4; ++i) acc[n][i] = part[n][i] = 0.f;
   const float zoff = AWQ ? -(float)(kOffset + a.zp) : -(float)kOffset;
   const uint4* xl = sx + (TP == 1 ? t : lane);
   const float* xsl = xs + (TP == 1 ? 0 : 2 * t);
 
-  auto flush = [&](const float* xg, const uint32_t (&s)[RT], const uint32_t (&z)[RT]) {  // xg: the group's sums
+  auto flush = [&](const float* xg, const char* w) {  // xg: the group's sums, w: its scale pairs
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float2 x;
@@ -178,20 +188,17 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
         x.x = x.y = *xg;
       else
         x = *reinterpret_cast<const float2*>(xg + n * 8);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const float2 sf = pair_f32(s[r]);
-        float (&o)[4] = acc[r][n];
-        float (&q)[4] = part[r][n];
-        if (!AWQ) {
-          const float2 zf = pair_f32(z[r]);
-          o[0] = fmaf(zf.x, x.x, o[0]), o[1] = fmaf(zf.x, x.y, o[1]);
-          o[2] = fmaf(zf.y, x.x, o[2]), o[3] = fmaf(zf.y, x.y, o[3]);
-        }
-        o[0] = fmaf(sf.x, fmaf(zoff, x.x, q[0]), o[0]), o[1] = fmaf(sf.x, fmaf(zoff, x.y, q[1]), o[1]);
-        o[2] = fmaf(sf.y, fmaf(zoff, x.x, q[2]), o[2]), o[3] = fmaf(sf.y, fmaf(zoff, x.y, q[3]), o[3]);
-        q[0] = q[1] = q[2] = q[3] = 0.f;
+      const float2 sf = pair_f32(*reinterpret_cast<const uint32_t*>(w));
+      float (&o)[4] = acc[n];
+      float (&q)[4] = part[n];
+      if (!AWQ) {
+        const float2 zf = pair_f32(*reinterpret_cast<const uint32_t*>(w + kGrp * 32));
+        o[0] = fmaf(zf.x, x.x, o[0]), o[1] = fmaf(zf.x, x.y, o[1]);
+        o[2] = fmaf(zf.y, x.x, o[2]), o[3] = fmaf(zf.y, x.y, o[3]);
       }
+      o[0] = fmaf(sf.x, fmaf(zoff, x.x, q[0]), o[0]), o[1] = fmaf(sf.x, fmaf(zoff, x.y, q[1]), o[1]);
+      o[2] = fmaf(sf.y, fmaf(zoff, x.x, q[2]), o[2]), o[3] = fmaf(sf.y, fmaf(zoff, x.y, q[3]), o[3]);
+      q[0] = q[1] = q[2] = q[3] = 0.f;
     }
   };
 
@@ -247,100 +254,65 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
     const Seg nxt = seg_of(nunit, nslab1);
     const uint4* xb = xl + (size_t)cur.b0 * 8 * kXW;
     const float* xg = xsl + cur.b0 * kGrp * TP;
-    for (int b = 0; b < cur.nb || b == 0; b += GB) {
-      const bool last = b + GB >= cur.nb;
-      const char* src = last ? nxt.q : cur.q + (size_t)(b + GB) * kBB;
-      const int left = last ? nxt.nb : cur.nb - b - GB;  // blocks to fetch from src
-      const size_t off = RT > 1 ? tile_off(1, last ? nunit : unit) : 0;
+    for (int b = 0; b < cur.nb; ++b) {
+      if (!__all_sync(0xffffffffu, mb_wait(&bar[slot], par, &abort_flag))) bad = true;
+      const char* wb = ring + slot * kBB;
 #pragma unroll
-      for (int j = 0; j < GB; ++j) {
-        const bool more = j < left;
-        const char* sq = src + j * kBB;
-        if (b + j < cur.nb) {  // uniform over the warp
+      for (int i = 0; i < 4; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(wb + lq + i * 512);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[RT][4];
+        for (int kb = 0; kb < 2; ++kb) {
+          uint4 x[NT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              w[r][0] = qw[j][i][r].x, w[r][1] = qw[j][i][r].y, w[r][2] = qw[j][i][r].z, w[r][3] = qw[j][i][r].w;
-              if (more) qw[j][i][r] = ld_stream(sq + (r ? off : 0) + lq + i * 512);
+          for (int n = 0; n < NT; ++n) x[n] = xb[(2 * i + kb) * kXW + n * 32];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            uint32_t f[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {  // rows g and g + 8, k in two halves
+              const uint32_t v = (h & 1) ? (kb ? w.w : w.z) : (kb ? w.y : w.x);
+              f[h] = nib_pair(__funnelshift_r(v, v, 4 * (2 * kt + (h >> 1))));
             }
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-              uint4 x[NT];
-#pragma unroll
-              for (int n = 0; n < NT; ++n) x[n] = xb[(2 * i + kb) * kXW + n * 32];
-#pragma unroll
-              for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                  uint32_t f[4];
-#pragma unroll
-                  for (int h = 0; h < 4; ++h) {  // rows g and g + 8, k in two halves
-                    const uint32_t v = w[r][(h & 1) * 2 + kb];
-                    f[h] = nib_pair(__funnelshift_r(v, v, 4 * (2 * kt + (h >> 1))));
-                  }
-#pragma unroll
-                  for (int n = 0; n < NT; ++n) mma16816(part[r][n], f, kt ? x[n].z : x[n].x, kt ? x[n].w : x[n].y);
-                }
-              if ((2 * i + kb) % FL == FL - 1) {
-                const int gi = (2 * i + kb) / FL;
-                flush(xg + gi * TP, sw[j][gi], zw[j][gi]);
-                if (more)
-#pragma unroll
-                  for (int r = 0; r < RT; ++r) {
-                    sw[j][gi][r] = ld_pair(sq + (r ? off : 0) + ls + gi * 32);
-                    if (!AWQ) zw[j][gi][r] = ld_pair(sq + (r ? off : 0) + ls + (kGrp + gi) * 32);
-                  }
-              }
-            }
+            for (int n = 0; n < NT; ++n) mma16816(part[n], f, kt ? x[n].z : x[n].x, kt ? x[n].w : x[n].y);
           }
-          xb += 8 * kXW;
-          xg += kGrp * TP;
-        } else if (more) {
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qw[j][i][r] = ld_stream(sq + (r ? off : 0) + lq + i * 512);
-#pragma unroll
-            for (int i = 0; i < kGrp; ++i) {
-              sw[j][i][r] = ld_pair(sq + (r ? off : 0) + ls + i * 32);
-              if (!AWQ) zw[j][i][r] = ld_pair(sq + (r ? off : 0) + ls + (kGrp + i) * 32);
-            }
+          if ((2 * i + kb) % FL == FL - 1) {
+            const int gi = (2 * i + kb) / FL;
+            flush(xg + gi * TP, wb + ls + gi * 32);
           }
         }
       }
+      xb += 8 * kXW;
+      xg += kGrp * TP;
+      __syncwarp();  // the place has been read
+      fetch();
+      if (++slot == p.ring) slot = 0, par ^= 1;
     }
     cur = nxt;
     if (nslab1 == 0) {  // the unit's last slab
       if (p.lk == 0 && p.lc == 0) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              store((((unit << lr) + wt) * RT + r) * 16 + g + (i >> 1) * 8, tok0 + n * 8 + 2 * t + (i & 1), acc[r][n][i]);
+          for (int i = 0; i < 4; ++i)
+            store(((unit << lr) + wt) * 16 + g + (i >> 1) * 8, tok0 + n * 8 + 2 * t + (i & 1), acc[n][i]);
       } else {
         // partial sums of the K slices, added in slice order (rank, then warp);
         // such a grid has a cluster per unit, so the buffer is written once
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              red[(warp * kCols + n * 8 + 2 * t + (i & 1)) * kColLd + r * 16 + g + (i >> 1) * 8] = acc[r][n][i];
+          for (int i = 0; i < 4; ++i)
+            red[(warp * kCols + n * 8 + 2 * t + (i & 1)) * kColLd + g + (i >> 1) * 8] = acc[n][i];
         if (c > 1)
           cluster_sync();
         else
           __syncthreads();
-        constexpr int kLrow = RT == 1 ? 4 : 5;  // log2 of kRows
-        const int lrows = lr + kLrow, step = kLinThreads << p.lc;
+        const int lrows = lr + 4, step = kLinThreads << p.lc;
         const int cols = min(kCols, a.T - tok0);
         for (int e = threadIdx.x + rank * kLinThreads; e < cols << lrows; e += step) {
-          const int row = e & ((1 << lrows) - 1), col = e >> lrows, w0 = row >> kLrow;
-          const float* at = red + (w0 * kCols + col) * kColLd + (row & (kRows - 1));
+          const int row = e & ((1 << lrows) - 1), col = e >> lrows, w0 = row >> 4;
+          const float* at = red + (w0 * kCols + col) * kColLd + (row & 15);
           float v = 0.f;
           for (int q = 0; q < c; ++q)
             for (int s = 0; s < ksw; ++s) v += ld_cluster(at + (s << lr) * kCols * kColLd, q, c);
@@ -348,48 +320,53 @@ __global__ void __launch_bounds__(kLinThreads, 2) k_linear(const LinArgs a, cons
         }
       }
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
     }
     unit = nunit;
     slab = nslab1;
   }
+  if (bad) {
+    if (a.err && lane == 0) atomicOr(a.err, 1);
+    drain_ring(bar, p.ring, issued, 0, 1);  // no copy is in flight when the CTA leaves
+  }
   if (c > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
 }
 
-constexpr int kLinSmemMax = 100 * 1024;  // two CTAs per SM
+constexpr int kLinSmemMax = 224 * 1024;  // one CTA per SM
 
-template <int FL, bool AWQ, int NT, int RT, int TP>
+template <int FL, bool AWQ, int NT, int TP>
 cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
   LinPlan p{};
   const int ntb = (a.T + NT * 8 - 1) / (NT * 8);
-  const int tg = (a.mt + RT - 1) / RT;
-  // K is split as long as every CTA stays resident at once (two per SM) and a
+  // K is split as long as every CTA stays resident at once (one per SM) and a
   // warp keeps a block: inside the CTA while its activations stay below half of
   // its weights, then over a cluster, then inside the CTA at any price.  A second
-  // round of CTAs costs more than the shorter slices give (T = 8, 11008 x 4096:
-  // 344 CTAs 17.5 us, 172 CTAs 10.3 us).
+  // round of CTAs costs more than the shorter slices give (T = 8, 11008 x 4096 with
+  // half as large CTAs: 17.5 us in two rounds, 16.0 us in one).
   int ksw = 1, c = 1;
   auto fits = [&](int w, int k) {
     const int rbt = kLinWarps / w;
-    return (long long)((tg + rbt - 1) / rbt) * ntb * k <= 2 * 148 && a.nb >= w * k;
+    return (long long)((a.mt + rbt - 1) / rbt) * ntb * k <= 148 && a.nb >= w * k;
   };
-  while (ksw < kLinWarps && TP * ksw * 2 <= 16 * RT && fits(2 * ksw, c)) ksw *= 2, ++p.lk;
+  while (ksw < kLinWarps && TP * ksw * 2 <= 16 && fits(2 * ksw, c)) ksw *= 2, ++p.lk;
   while (c < 8 && fits(ksw, 2 * c)) c *= 2, ++p.lc;
   while (ksw < kLinWarps && fits(2 * ksw, c)) ksw *= 2, ++p.lk;
   const int rbt = kLinWarps / ksw;
-  p.units = (tg + rbt - 1) / rbt;
+  p.units = (a.mt + rbt - 1) / rbt;
   const bool split = ksw > 1 || c > 1;
-  const int red = split ? kLinWarps * NT * 8 * (RT * 16 + 4) * 4 : 0;
+  const int red = split ? kLinWarps * NT * 8 * (16 + 4) * 4 : 0;
   const int per_block = TP * 4 * 8 * 16 + 8 / FL * TP * 4;
   const int share = (a.nb + c - 1) / c;
-  p.bps = std::max(1, std::min(share, (kLinSmemMax - red) / per_block));
+  // the activations get what leaves two places of each warp's ring, the ring the rest
+  constexpr int place = kLinWarps * lin_block_bytes(FL, !AWQ);
+  p.bps = std::max(1, std::min(share, (kLinSmemMax - red - 2 * place) / per_block));
   p.nslab = (share + p.bps - 1) / p.bps;
-  const int smem = p.bps * per_block + red;
-  const auto kernel = k_linear<FL, AWQ, NT, RT, TP>;
+  p.ring = std::min(kRingMax, (kLinSmemMax - red - p.bps * per_block) / place);
+  static_assert(2 * place + kLinWarps * NT * 8 * (16 + 4) * 4 + TP * 4 * 8 * 16 + 8 / FL * TP * 4 <= kLinSmemMax, "");
+  const int smem = p.ring * place + p.bps * per_block + red;
+  const auto kernel = k_linear<FL, AWQ, NT, TP>;
   static bool attr[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -398,7 +375,7 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr[dev] = true;
   }
-  const long long gx = (split ? p.units : std::min(p.units, std::max(1, 148 * 2 / ntb))) * (long long)c;
+  const long long gx = (split ? p.units : std::min(p.units, std::max(1, 148 / ntb))) * (long long)c;
   if (gx > 0x7FFFFFFFll || ntb > 65535) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)gx, (unsigned)ntb);
@@ -418,9 +395,9 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
 
 template <int FL, bool AWQ>
 cudaError_t launch_fl(const LinArgs& a, cudaStream_t st) {
-  if (a.T == 1) return launch_shape<FL, AWQ, 1, 1, 1>(a, st);
-  if (a.T <= 8) return launch_shape<FL, AWQ, 1, 1, 8>(a, st);
-  return launch_shape<FL, AWQ, 2, 2, 16>(a, st);
+  if (a.T == 1) return launch_shape<FL, AWQ, 1, 1>(a, st);
+  if (a.T <= 8) return launch_shape<FL, AWQ, 1, 8>(a, st);
+  return launch_shape<FL, AWQ, 2, 16>(a, st);
 }
 
 // One 32-bit word of the stream per thread: words of a block (rows past M and
@@ -466,12 +443,17 @@ cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st) {
 }
 
 cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st) {
-  // From 17 tokens on mma.sync, which needs the weights dequantised once per 16
-  // tokens, is slower on every shape measured (K = 4096; T = 24, groups of 128:
-  // 9.9 against 35 us at 4096 rows, 87 against 88 at 60000); at 16 tokens it is
-  // faster for wide matrices and small groups (52 against 81 us at 60000 rows, 60
-  // against 154 with groups of 32) and about equal otherwise.
-  if (a.T > 16 && (!awq || a.zp < 16)) return launch_linear_umma(a, fl, awq, st);
+  // mma.sync needs the weights dequantised once per 16 tokens, tcgen05's CTAs take
+  // 64 tokens against 128 rows.  From 17 tokens on the latter is faster up to some
+  // 100000 rows, and always from 33 (T = 24, groups of 128: 4096 x 4096 8.5 against
+  // 10.6 us, 60000 x 4096 67 against 80, 100000 x 2048 61.2 against 59.4, 248320 x
+  // 2048 142 against 130); from 9 tokens on while its tiles need about one round of
+  // CTAs, half that with small groups (T = 16, K = 4096: 4096 rows 8.0 against 15.6
+  // us, 11008 rows 14.8 against 16.5, 30000 rows 30.3 against 29.3; groups of 32: 4096
+  // rows 10.2 against 16.9, 11008 rows 23.8 against 19.2).
+  const int tiles = (a.mt + 7) / 8;
+  const bool umma = a.T > 32 || (a.T > 16 && tiles <= 768) || (a.T > 8 && tiles <= (fl == 4 ? 148 : 64));
+  if (umma && (!awq || a.zp < 16)) return launch_linear_umma(a, fl, awq, st);
   switch (fl) {
     case 1: return awq ? launch_fl<1, true>(a, st) : launch_fl<1, false>(a, st);
     case 2: return awq ? launch_fl<2, true>(a, st) : launch_fl<2, false>(a, st);
