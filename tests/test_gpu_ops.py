@@ -23,6 +23,7 @@ BF16, F32 = torch.bfloat16, torch.float32
 def cuda_ready():
     assert torch.cuda.is_available(), "gpu tests need a CUDA device"
     yield
+    torch.cuda.empty_cache()
 
 
 def gen(seed):
@@ -764,3 +765,156 @@ def test_binding_refuses_wrong_tensors():
         L.BeamReorder([flat[:2]], [flat[1:]], 2, 4, 4).run(torch.zeros((2, 4), dtype=torch.int32, device="cuda"))
     torch.cuda.synchronize()
     assert bool((y == 5).all()) and bool((s == 0).all())
+
+
+# --------------------------------------------- shapes and calls at the edges
+
+@pytest.mark.parametrize("M,K,gs", [(130, 640, 32), (300, 1408, 64), (300, 1376, 32), (700, 896, 128), (129, 2944, 128)])
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("pad", [0, 8, 5])
+def test_linear_k_split_at_odd_steps(M, K, gs, asym, pad):
+    """An odd number of 128-wide steps over several CTAs, aligned and unaligned
+    rows, one to three blocks of tokens."""
+    w = Weight(M, K, gs, asym, seed=M + K + gs)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    for T in (9, 12, 20, 48, 64, 65, 150):
+        x = torch.randn((T, K + pad), generator=gen(T), device="cuda").to(BF16)[:, :K]
+        y = x.double() @ w.w.t()
+        got = run_linear(lin, w, x, T, F32)
+        close(got, y, w.tol(x, y, F32), f"T={T}")
+        assert torch.equal(got, run_linear(lin, w, x, T, F32))
+    lin.status(stream())
+    lin.close()
+
+
+@pytest.mark.parametrize("T", [1, 8, 16, 30])
+@pytest.mark.parametrize("gs", [32, 128])
+def test_linear_on_two_streams_at_once(T, gs):
+    """One handle, two streams: each call its own answer."""
+    w = Weight(6000, 1024, gs, True, seed=21)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    xs = [torch.randn((T, w.K), generator=gen(i), device="cuda").to(BF16) for i in range(2)]
+    want = [run_linear(lin, w, x, T, F32) for x in xs]
+    st = [torch.cuda.Stream() for _ in range(2)]
+    ys = [[torch.empty((T, w.M), device="cuda") for _ in range(10)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for j in range(2):
+            lin.forward(xs[j], T, ys[j][i], stream=st[j])
+    torch.cuda.synchronize()
+    for j in range(2):
+        assert all(torch.equal(y, want[j]) for y in ys[j])
+    lin.status(stream())
+
+
+@pytest.mark.parametrize("T", [1, 7, 12, 40])
+def test_rows_past_the_last_stay(T):
+    """Buffers with more rows than the call: the others keep their bits."""
+    w = Weight(200, 256, 32, False, seed=31)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    x = torch.randn((T + 9, w.K), generator=gen(1), device="cuda").to(BF16)
+    x[T:] = float("nan")
+    y = torch.full((T + 9, w.M), 5.0, dtype=BF16, device="cuda")
+    lin.forward(x, T, y, stream=stream())
+    op = L.ResidualNorm(w.K, pre="rms")
+    r = torch.randn((T + 9, w.K), generator=gen(2), device="cuda").to(BF16)
+    ro, no = torch.full_like(r, 5.0), torch.full_like(r, 5.0)
+    op.forward(T, x, r, ro, no, stream=stream())
+    torch.cuda.synchronize()
+    for v in (y, ro, no):
+        assert bool((v[T:] == 5).all()) and bool(torch.isfinite(v[:T]).all())
+
+
+def far_rows(T, n, dtype=BF16, value=None):
+    """[T, n] rows 2^28 + 8 elements apart: from row 16 on, offsets pass 32 bits."""
+    big = torch.empty((T, (1 << 28) + 8), dtype=dtype, device="cuda")
+    v = big[:, :n]
+    if value is not None:
+        v.copy_(value)
+    return v
+
+
+@pytest.mark.parametrize("gs", [32, 128])
+def test_linear_offsets_past_32_bits(gs):
+    T = 20
+    w = Weight(150, 256, gs, True, seed=41)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    x = torch.randn((T, w.K), generator=gen(3), device="cuda").to(BF16)
+    xf, yf = far_rows(T, w.K, value=x), far_rows(T, w.M)
+    lin.forward(xf, T, yf, R=yf.copy_(torch.ones((T, w.M), device="cuda")), stream=stream())
+    y = torch.empty((T, w.M), dtype=BF16, device="cuda")
+    lin.forward(x, T, y, R=torch.ones_like(y), stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(yf, y)
+    for t in (1, 8):  # the kernel of few tokens, its rows far behind one another
+        y = torch.empty((t, w.M), dtype=BF16, device="cuda")
+        lin.forward(x[:t], t, y, stream=stream())
+        lin.forward(xf[20 - t * 2::2] if t == 8 else xf[:1], t, yf, stream=stream())
+        want = torch.empty_like(y)
+        lin.forward(x[20 - t * 2::2].contiguous() if t == 8 else x[:1], t, want, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(yf[:t], want)
+
+
+def test_norm_offsets_past_32_bits():
+    T, H = 20, 300
+    op = L.ResidualNorm(H, post="rms", pre="layer")
+    b, r = (torch.randn((T, H), generator=gen(i), device="cuda").to(BF16) for i in (4, 5))
+    ro, no = torch.empty_like(r), torch.empty_like(r)
+    op.forward(T, b, r, ro, no, stream=stream())
+    bf, rf, nf = far_rows(T, H, value=b), far_rows(T, H, value=r), far_rows(T, H)
+    op.forward(T, bf, rf, rf, nf, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(rf, ro) and torch.equal(nf, no)
+
+
+def test_select_offsets_past_32_bits():
+    B, W, V = 4, 5, 5000
+    x = torch.randn((B * W, V), generator=gen(6), device="cuda").to(BF16)
+    scores = torch.randn((B, W), generator=gen(7), device="cuda")
+    want = run_select(x, scores, None, -1, 6)
+    got = run_select(far_rows(B * W, V, value=x), scores, None, -1, 6)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_reorder_offsets_past_32_bits():
+    W, row = 4, 1200 * 1000 * 1000 + 48
+    src = torch.empty((1, W, row), dtype=torch.uint8, device="cuda")
+    for i in range(W):
+        src[0, i] = torch.randint(0, 256, (1 << 20,), generator=gen(i), device="cuda", dtype=torch.uint8).repeat(
+            row // (1 << 20) + 1)[:row]
+    dst = torch.zeros_like(src)
+    parent = torch.tensor([[3, 0, 3, 2]], dtype=torch.int32, device="cuda")
+    L.BeamReorder([src], [dst], 1, W, W).run(parent, stream=stream())
+    torch.cuda.synchronize()
+    for i, p in enumerate((3, 0, 3, 2)):
+        assert torch.equal(dst[0, i], src[0, p])
+
+
+def test_captured_calls_with_their_own_workspaces():
+    """Two captured selections, each with its own workspace, replayed in turn
+    and at once on two streams."""
+    B, W, V, k = 3, 6, 30011, 6
+    cases = []
+    for i in range(2):
+        x = torch.randn((B * W, V), generator=gen(50 + i), device="cuda").to(BF16)
+        scores = torch.randn((B, W), generator=gen(60 + i), device="cuda")
+        want = run_select(x, scores, None, -1, k)
+        bs = L.BeamSearch(B, W, V, k)
+        ws = torch.empty(bs.workspace_bytes(), device="cuda", dtype=torch.uint8)
+        outs = [torch.zeros((B, k), dtype=torch.int32, device="cuda"), torch.zeros((B, k), dtype=torch.int32, device="cuda"),
+                torch.zeros((B, k), device="cuda"), torch.zeros((B, k), dtype=torch.uint8, device="cuda")]
+        st = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=st):
+            bs.select(x, scores, outs[0], outs[1], outs[2], ws, ws.numel(), finished_out=outs[3],
+                      stream=torch.cuda.current_stream())
+        cases.append((graph, want, outs, torch.cuda.Stream(), (x, scores, ws, bs)))
+    for _ in range(20):
+        for graph, _, _, st, _ in cases:
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, want, outs, _, _ in cases:
+        assert all(torch.equal(a, b) for a, b in zip(want, outs))

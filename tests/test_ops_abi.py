@@ -175,3 +175,7 @@ def test_accepted_calls_need_a_device():
     t = (L.ReorderTensor * 3)(tensor(), tensor(src=3 * A, dst=3 * A),
                               tensor(src=4 * A, dst=5 * A, n_seg=3, seg_stride=512, src_stride=64, dst_stride=64))
     assert lib.llmoc_beam_reorder(t, 3, 9 * A, 2, 4, 4, 0, None) == 2
+
+
+def test_linear_status_refuses_a_null_handle():
+    assert lib.llmoc_int4_linear_status(None, None) == 1 and "null linear" in L.last_error()
