@@ -317,7 +317,9 @@ LLMOC_API llmoc_status llmoc_moe_noalloc_status(const llmoc_moe_layer* layer, in
  * beam search with the reordering of the beams' states.  Each call works on
  * `device` (or its handle's device) whatever the current one is, restores the
  * current device, allocates nothing, and can be captured into a CUDA graph.
- * `stream` must belong to that device.  Row strides (ld*) count elements. */
+ * `stream` must belong to that device.  Row strides (ld*) count elements.  A
+ * handle may be used on several streams at once; a workspace serves one call at
+ * a time, so two captured graphs that may run at once need one each. */
 
 enum { LLMOC_NORM_NONE = 0, LLMOC_NORM_RMS = 1, LLMOC_NORM_LAYER = 2 };
 enum { LLMOC_ACT_NONE = 0, LLMOC_ACT_SIGMOID = 1 };
@@ -338,17 +340,20 @@ LLMOC_API void llmoc_int4_linear_destroy(llmoc_int4_linear* linear);
 /* Bytes of resident weights one product streams (packed q + fp16 scales / zeros, with the padding to 16 rows x 64 k). */
 LLMOC_API size_t llmoc_int4_linear_weight_bytes(const llmoc_int4_linear* linear);
 /* Y[t, m] = sum_k W[m, k] X[t, k] (+ R[t, m]), t < T, one rounding to y_dtype
- * (LLMOC_DTYPE_*): products of bf16 activations with exact integers, group
- * sums and their scaled sum in fp32, a fixed order of summation.  X, R bf16; R
- * may be null, and may be Y itself (bf16, ldr = ldy).  X overlaps neither R
- * nor Y.  T = 0 does nothing. */
+ * (LLMOC_DTYPE_*): products of bf16 activations with exact integers (or, from 9
+ * tokens on, with the exact scaled weights as two bf16 terms), sums in fp32, a
+ * fixed order of summation for given T.  A token with a non-finite activation
+ * gets non-finite outputs and changes no other token's.  X, R bf16; R may be
+ * null, and may be Y itself (bf16, ldr = ldy).  X overlaps neither R nor Y.
+ * T = 0 does nothing. */
 LLMOC_API llmoc_status llmoc_int4_linear_forward(const llmoc_int4_linear* linear, const uint16_t* X, int64_t ldx, int T,
                                                  const uint16_t* R, int64_t ldr, void* Y, int64_t ldy, int y_dtype,
                                                  void* stream);
 
 /* Synchronizes `stream`, reads and clears the handle's device error word:
  * LLMOC_ERR_TIMEOUT when one of a forward's bounded device-side waits gave up
- * since the last such call (its outputs are then not valid), else LLMOC_OK. */
+ * since the last such call (its outputs are then not valid), else LLMOC_OK.
+ * LLMOC_ERR_INVALID while the stream is being captured. */
 LLMOC_API llmoc_status llmoc_int4_linear_status(llmoc_int4_linear* linear, void* stream);
 
 /* Between two blocks of a decoder (the reference's rmsnorm_w16 and vec_add

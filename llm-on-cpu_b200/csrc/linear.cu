@@ -363,7 +363,9 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
   constexpr int place = kLinWarps * lin_block_bytes(FL, !AWQ);
   p.bps = std::max(1, std::min(share, (kLinSmemMax - red - 2 * place) / per_block));
   p.nslab = (share + p.bps - 1) / p.bps;
-  p.ring = std::min(kRingMax, (kLinSmemMax - red - p.bps * per_block) / place);
+  const int ncl = !split ? std::min(p.units, std::max(1, 148 / ntb)) : p.units;
+  const long long mine = (long long)((p.units + ncl - 1) / ncl) * ((share + ksw - 1) / ksw);  // a warp's blocks at most
+  p.ring = (int)std::min<long long>(std::min(kRingMax, (kLinSmemMax - red - p.bps * per_block) / place), mine);
   static_assert(2 * place + kLinWarps * NT * 8 * (16 + 4) * 4 + TP * 4 * 8 * 16 + 8 / FL * TP * 4 <= kLinSmemMax, "");
   const int smem = p.ring * place + p.bps * per_block + red;
   const auto kernel = k_linear<FL, AWQ, NT, TP>;
@@ -375,7 +377,7 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr[dev] = true;
   }
-  const long long gx = (split ? p.units : std::min(p.units, std::max(1, 148 / ntb))) * (long long)c;
+  const long long gx = ncl * (long long)c;
   if (gx > 0x7FFFFFFFll || ntb > 65535) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)gx, (unsigned)ntb);

@@ -280,6 +280,11 @@ llmoc_status llmoc_int4_linear_status(llmoc_int4_linear* L, void* stream) {
   if (!L) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": null linear");
   OnDevice od(L->device);
   if (!od.ok) return no_device(who, L->device);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing((cudaStream_t)stream, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the stream is being captured");
+  }
   int word = 0;
   cudaError_t e = cudaMemcpyAsync(&word, L->err, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(L->err, 0, 4, (cudaStream_t)stream);

@@ -918,3 +918,40 @@ def test_captured_calls_with_their_own_workspaces():
     torch.cuda.synchronize()
     for _, want, outs, _, _ in cases:
         assert all(torch.equal(a, b) for a, b in zip(want, outs))
+
+
+@pytest.mark.parametrize("T", [5, 12, 40])
+@pytest.mark.parametrize("gs", [32, 64, 128])
+def test_linear_non_finite_rows_with_zeros(T, gs):
+    """With zeros too, whose product with the group sums is apart: a token with
+    inf or NaN changes no other token's bits and has no finite output."""
+    w = Weight(200, 512, gs, True, seed=12)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    x = torch.randn((T, 512), generator=gen(10), device="cuda").to(BF16)
+    clean = run_linear(lin, w, x, T, F32)
+    x[1, 100] = float("inf")
+    x[2, 7] = -float("inf")
+    x[T - 1, 3] = float("nan")
+    y = run_linear(lin, w, x, T, F32)
+    keep = [t for t in range(T) if t not in (1, 2, T - 1)]
+    assert torch.equal(y[keep], clean[keep])
+    for t, k in ((1, 100), (2, 7), (T - 1, 3)):
+        assert not bool(torch.isfinite(y[t, w.w[:, k] != 0]).any())
+
+
+def test_linear_status_refuses_a_captured_stream():
+    w = Weight(64, 128, 32, False, seed=13)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    x = torch.randn((12, 128), generator=gen(1), device="cuda").to(BF16)
+    want = run_linear(lin, w, x, 12, F32)
+    y = torch.zeros_like(want)
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        lin.forward(x, 12, y, stream=torch.cuda.current_stream())
+        with pytest.raises(L.LlmocError, match="captured"):
+            lin.status(torch.cuda.current_stream())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    lin.status(stream())
