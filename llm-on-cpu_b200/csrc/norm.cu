@@ -76,7 +76,8 @@ __device__ __forceinline__ float row_sum(float v, float* sh) {
   return v;
 }
 
-constexpr int kNormMinThreads = 128;  // rows of one warp share a CTA of four
+// threads of a CTA: a row's, or four rows of one warp
+constexpr int norm_threads(int G) { return G > 32 ? G : 128; }
 
 // How a thread holds its columns of an operand: eight neighbours per 16-byte
 // access (kVec), all of them bf16 and kept packed until used (kBf16), or columns
@@ -96,13 +97,13 @@ struct Held<kBf16, VPT> {
 // waits for memory once.  Without, the weights are fetched where they are used,
 // which leaves registers for more rows per SM.
 template <int G, int VPT, int MODE, bool HOLD>
-__global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads, (MODE == kBf16 || !HOLD) && VPT <= 2 ? 1024 / (G > kNormMinThreads ? G : kNormMinThreads) : 1)
+__global__ void __launch_bounds__(norm_threads(G), (MODE == kBf16 || !HOLD) && VPT <= 2 ? 1024 / norm_threads(G) : 1)
     k_norm(const __grid_constant__ NormArgs a) {
   constexpr int N = 8 * VPT;
   using Row = Held<MODE, VPT>;
   __shared__ float sh[8][32];  // one slice per reduction of a row: no second barrier between two of them
   const int tid = G > 32 ? threadIdx.x : threadIdx.x & 31;
-  const int row = G > 32 ? blockIdx.x : blockIdx.x * (kNormMinThreads / 32) + (threadIdx.x >> 5);
+  const int row = G > 32 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
   grid_dep_wait();
   grid_dep_release();
   if (row >= a.T) return;  // whole warps, and only where no barrier follows (G == 32)
@@ -272,14 +273,18 @@ __global__ void __launch_bounds__(G > kNormMinThreads ? G : kNormMinThreads, (MO
   }
 }
 
+// every operand read or written in rows is bf16
+bool all_bf16(const NormArgs& a) {
+  return !(a.block && a.block_f32) && !((a.res || a.res_out) && a.res_f32) && !(a.out && a.out_f32) &&
+         !((a.post_w || a.post_b || a.pre_w || a.pre_b) && a.w_f32) && !(a.gate && a.gate_col && a.gate_f32);
+}
+
 template <int G, int VPT, bool HOLD>
 cudaError_t launch_held(const NormArgs& a, cudaStream_t st) {
-  const dim3 block(std::max(G, kNormMinThreads));
+  const dim3 block(norm_threads(G));
   const dim3 grid((unsigned)(G > 32 ? a.T : (a.T + 3) / 4));
   if (!a.vec) return launch_pdl(k_norm<G, VPT, kScalar, HOLD>, grid, block, 0, st, a);
-  const bool bf16 = !(a.block && a.block_f32) && !((a.res || a.res_out) && a.res_f32) && !(a.out && a.out_f32) &&
-                    !((a.post_w || a.post_b || a.pre_w || a.pre_b) && a.w_f32) && !(a.gate && a.gate_col && a.gate_f32);
-  if (bf16) return launch_pdl(k_norm<G, VPT, kBf16, VPT < 4>, grid, block, 0, st, a);
+  if (all_bf16(a)) return launch_pdl(k_norm<G, VPT, kBf16, VPT < 4>, grid, block, 0, st, a);
   return launch_pdl(k_norm<G, VPT, kVec, HOLD>, grid, block, 0, st, a);
 }
 
@@ -298,6 +303,21 @@ cudaError_t launch_g(const NormArgs& a, cudaStream_t st) {
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   const bool few = !a.vec && a.T <= 2 * 148;  // single-column accesses: fewer of them a thread
   if (a.H <= 256) return launch_g<32, 1>(a, st);
+  // Many rows of bf16: more columns a thread leave fewer threads to meet in a
+  // row's reductions and as many bytes in flight per SM.  16 columns from two rows
+  // per SM on (1000 x 2048 5.2 -> 4.5 us, 8192 x 512 15.9 -> 8.9), 32 columns of
+  // wide rows from 1024 rows on (8192 x 4096 53.5 -> 44.6, 4096 x 8192 62 -> 47.5,
+  // 8192 x 2048 27.4 -> 24.4; 500 x 4096 4.8 -> 5.1 without that rule).  64 columns
+  // are slower again (48.5 us at 8192 x 4096).  Mixed types unpack into twice the
+  // registers and lose by it (fp32 residual, 8192 x 4096: 92 -> 138 us).
+  if (a.vec && a.T > 2 * 148 && all_bf16(a)) {
+    const bool wide = a.T > 1024;
+    if (a.H <= 512) return launch_g<32, 2>(a, st);
+    if (a.H <= 1024) return launch_g<64, 2>(a, st);
+    if (a.H <= 2048) return wide ? launch_g<64, 4>(a, st) : launch_g<128, 2>(a, st);
+    if (a.H <= 4096 && wide) return launch_g<128, 4>(a, st);
+    if (a.H <= 8192 && wide) return launch_g<256, 4>(a, st);
+  }
   if (a.H <= 1024) return launch_g<128, 1>(a, st);
   if (a.H <= 2048) return launch_g<256, 1>(a, st);
   if (a.H <= 4096) return few ? launch_g<512, 1>(a, st) : launch_g<256, 2>(a, st);

@@ -955,3 +955,21 @@ def test_linear_status_refuses_a_captured_stream():
     torch.cuda.synchronize()
     assert torch.equal(y, want)
     lin.status(stream())
+
+
+@pytest.mark.parametrize("H", [200, 264, 512, 520, 1024, 1032, 2048, 2056, 4096, 4104, 5120, 8192, 8200])
+@pytest.mark.parametrize("T", [297, 1025])
+@pytest.mark.parametrize("rdt", [BF16, F32])
+def test_norm_many_rows(H, T, rdt):
+    """Enough rows for every variant of a wide batch."""
+    c = norm_config(H, "rms", "layer", BF16, seed=H)
+    op = L.ResidualNorm(H, **c)
+    g = gen(T + H)
+    b = (torch.randn((T, H), generator=g, device="cuda") * 2 + 0.5).to(BF16)
+    r = (torch.randn((T, H), generator=g, device="cuda") * 3 - 0.25).to(rdt)
+    ro, no = torch.empty_like(r), torch.empty((T, H), dtype=BF16, device="cuda")
+    op.forward(T, b, r, ro, no, stream=stream())
+    torch.cuda.synchronize()
+    wr, er, wn, en = ref_norm(b, r, None, c)
+    check_rows(ro, wr, er, "residual")
+    check_rows(no, wn, en, "norm")
