@@ -14,7 +14,10 @@
 // for few rows, by the launch and the chain load -> reduce -> reduce -> store.
 // A group of G threads holds a whole row in registers, so both norms need no
 // second read; the variance of a layer norm is the centred sum over those
-// registers.
+// registers.  8192 x 4096 bf16 rows with a gate per token take 44.7 us, 6.0 TB/s,
+// 0.93 of a plain copy's rate; 129 x 5001 with an fp32 residual, whose odd width
+// allows single columns only, 7.5 us; one row of 2048 2.1 us.  Rows copied ahead in
+// bulk by CTAs that stay (59.6 us) were slower than more CTAs in flight.
 #include <algorithm>
 #include <cfloat>
 #include <string>
