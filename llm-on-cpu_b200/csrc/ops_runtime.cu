@@ -516,6 +516,12 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
   if (!workspace || workspace_bytes < llmoc_beam_workspace_bytes(d))
     return refuse(LLMOC_ERR_WORKSPACE, std::string(who) + ": workspace too small");
   if (!aligned(workspace, 8)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace is not aligned to 8");
+  const long long used = (long long)llmoc_beam_workspace_bytes(d);
+  const Rows wr{workspace, used, used, 1};
+  for (const Rows& r : in)
+    if (overlap(wr, r)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace overlaps an input");
+  for (const Rows& r : outs)
+    if (overlap(wr, r)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace overlaps an output");
   OnDevice od(device);
   if (!od.ok) return no_device(who, device);
   BeamArgs a{};

@@ -179,3 +179,8 @@ def test_accepted_calls_need_a_device():
 
 def test_linear_status_refuses_a_null_handle():
     assert lib.llmoc_int4_linear_status(None, None) == 1 and "null linear" in L.last_error()
+
+
+@pytest.mark.parametrize("ws", [A, 2 * A, 3 * A, 4 * A, 5 * A])
+def test_beam_workspace_apart_from_operands(ws):
+    assert select(beam(), ws=ws) == 1 and "workspace overlaps" in L.last_error()
