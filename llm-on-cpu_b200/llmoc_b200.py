@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 from typing import Optional, Sequence
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -173,9 +174,9 @@ _SIGS = {
     "llmoc_int4_linear_weight_bytes": (_sz, [_vp]),
     "llmoc_int4_linear_status": (_i, [_vp, _vp]),
     "llmoc_int4_linear_forward": (_i, [_vp, _vp, C.c_int64, _i, _vp, C.c_int64, _vp, C.c_int64, _i, _vp]),
-    "llmoc_norm_residual": (_i, [C.POINTER(NormDesc), C.POINTER(NormIO), _i, _i, _vp]),
+    "llmoc_norm_residual": (_i, [C.POINTER(NormDesc), _vp, _i, _i, _vp]),  # io: a NormIO by reference or its bytes
     "llmoc_moe_block_workspace_bytes": (_sz, [_vp, _i]),
-    "llmoc_moe_forward_block": (_i, [_vp, C.POINTER(NormDesc), C.POINTER(NormDesc), C.POINTER(NormIO), _i, _vp, _sz,
+    "llmoc_moe_forward_block": (_i, [_vp, C.POINTER(NormDesc), C.POINTER(NormDesc), _vp, _i, _vp, _sz,
                                      _vp]),
     "llmoc_beam_workspace_bytes": (_sz, [C.POINTER(BeamDesc)]),
     "llmoc_beam_select": (_i, [C.POINTER(BeamDesc), _vp, C.c_int64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i,
@@ -331,7 +332,7 @@ class MoeLayer:
         """The MoE block on its residual stream: before's pre norm, the layer,
         then after's post norm, gate, scales, residual add and pre norm."""
         io = after.io(T, None, residual, residual_out, norm_out, gate)
-        check(lib.llmoc_moe_forward_block(self.handle, C.byref(before.desc), C.byref(after.desc), C.byref(io), T,
+        check(lib.llmoc_moe_forward_block(self.handle, C.byref(before.desc), C.byref(after.desc), io, T,
                                           ptr(ws), ws_bytes, stream_ptr(stream)), "llmoc_moe_forward_block")
 
     def route(self, X, T: int, ws, ws_bytes: int, stream=None) -> None:
@@ -411,13 +412,15 @@ def _device(x, device: int, what: str) -> int:
 def _rows(x, rows: int, cols: int, device: int, what: str):
     """(address, row stride) of a [>= rows, cols] tensor with adjacent columns."""
     shape, stride = x.shape, x.stride()
+    if len(shape) == 2:
+        (n, c), (ld, step) = shape, stride
+        if n >= rows and c == cols and (step == 1 or cols == 1) and x.get_device() == device:
+            return x.data_ptr(), ld if rows > 1 or ld > cols else cols
     if len(shape) != 2 or shape[0] < rows or shape[1] != cols:
         raise LlmocError(f"{what}: shape {tuple(shape)}, not [{rows}, {cols}]")
     if stride[1] != 1 and cols > 1:
         raise LlmocError(f"{what}: columns are not adjacent in memory")
-    if x.get_device() != device:
-        raise LlmocError(f"{what} is on {x.device}, not on cuda:{device}")
-    return x.data_ptr(), stride[0] if rows > 1 else max(stride[0], cols)
+    raise LlmocError(f"{what} is on {x.device}, not on cuda:{device}")
 
 
 class Int4Linear:
@@ -472,6 +475,10 @@ class Int4Linear:
             pass
 
 
+_NORM_IO = struct.Struct("PqPqPqPqPqqiiii").pack  # a NormIO's bytes, without the cost of filling one
+assert struct.calcsize("PqPqPqPqPqqiiii") == C.sizeof(NormIO)
+
+
 class ResidualNorm:
     """The norm after a block, its gate and scale, the residual add and the
     norm before the next block, in one pass (llmoc_norm_residual)."""
@@ -499,9 +506,10 @@ class ResidualNorm:
                              residual_scale, self.ACTS[gate_act])
         self._desc = C.byref(self.desc)
 
-    def io(self, T: int, block, residual, residual_out, norm_out, gate) -> NormIO:
+    def io(self, T: int, block, residual, residual_out, norm_out, gate) -> bytes:
+        """The operands as a llmoc_norm_io."""
         H, dev = self.hidden, self.device
-        b = r = ro = no = None
+        b = r = ro = no = 0
         ldb = ldr = ldro = ldno = 0
         bdt = rdt = ndt = DTYPE_BF16
         if block is not None:
@@ -514,21 +522,21 @@ class ResidualNorm:
                 raise LlmocError("residual and residual_out differ in type")
         if norm_out is not None:
             (no, ldno), ndt = _rows(norm_out, T, H, dev, "norm_out"), _dtype(norm_out, "norm_out")
-        g, gr, gc, gdt = None, 0, 0, DTYPE_BF16
+        g, gr, gc, gdt = 0, 0, 0, DTYPE_BF16
         if gate is not None:  # [T, H], [1, H], [T, 1] or [1, 1]
             if gate.dim() != 2 or (gate.shape[0] != 1 and gate.shape[0] < T) or gate.shape[1] not in (1, H):
                 raise LlmocError(f"gate: shape {tuple(gate.shape)}, not [{T} or 1, {H} or 1]")
             g, gdt = _device(gate, dev, "gate"), _dtype(gate, "gate")
             gr = gate.stride(0) if gate.shape[0] > 1 else 0
             gc = gate.stride(1) if gate.shape[1] > 1 else 0
-        return NormIO(b, ldb, r, ldr, ro, ldro, no, ldno, g, gr, gc, bdt, rdt, ndt, gdt)
+        return _NORM_IO(b, ldb, r, ldr, ro, ldro, no, ldno, g, gr, gc, bdt, rdt, ndt, gdt)
 
     def forward(self, T: int, block, residual, residual_out, norm_out, gate=None, stream=None) -> None:
         """residual_out = residual_scale * residual + block_scale * act(gate) *
         post(block), norm_out = pre(that); any operand may be None where the
         desc needs none."""
         io = self.io(T, block, residual, residual_out, norm_out, gate)
-        st = lib.llmoc_norm_residual(self._desc, C.byref(io), T, self.device, stream_ptr(stream))
+        st = lib.llmoc_norm_residual(self._desc, io, T, self.device, stream_ptr(stream))
         if st:
             check(st, "llmoc_norm_residual")
 
@@ -546,6 +554,8 @@ class BeamSearch:
         return int(lib.llmoc_beam_workspace_bytes(C.byref(self.desc)))
 
     def _plain(self, x, shape, kind: int, what: str):
+        if _KIND.get(x.dtype) == kind and x.shape == shape and x.is_contiguous() and x.get_device() == self.device:
+            return x.data_ptr()
         if x.shape != shape or _kind(x) != kind or not x.is_contiguous():
             raise LlmocError(f"{what}: not a contiguous {_KINDS[kind]} tensor of shape {shape}")
         if x.get_device() != self.device:
