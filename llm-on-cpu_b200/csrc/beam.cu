@@ -24,12 +24,12 @@
 //                 a bound, what reaches it, ranked by counting.
 //
 // What bounds it (graph replay): 32 sequences x 8 beams x 248320 bf16 logits take
-// 46.8 us, 2.7 TB/s; of those the exponentials alone, 4 a clock and scheduler, are
+// 46.4 us, 2.7 TB/s; of those the exponentials alone, 4 a clock and scheduler, are
 // 14 us, and with the unpacking, sums and comparisons a scheduler needs some 360
 // cycles for a warp's 1024 elements.  Rows copied ahead in bulk took 48.3 us: it
-// does not wait for memory.  8 x 4 x 131072 fp32 with 8 candidates take 16.0 us
-// (1.0 TB/s), 1 x 4 x 32003 8.9 us, of which the two launches and a chain of load,
-// first bound, list and merge are nearly all.
+// does not wait for memory.  8 x 4 x 131072 fp32 with 8 candidates take 15.5 us
+// (1.1 TB/s), 1 x 4 x 32003 8.4 us, of which the two launches and a chain of load,
+// first bound, list and merge are nearly all; the merge has 3 to 5 us of each.
 //
 // Order of summation is fixed by the slice and thread numbers alone, so equal
 // rows get equal bits and ties resolve by index.
@@ -121,18 +121,24 @@ __device__ __forceinline__ float logit_at(const BeamArgs& a, long long i) {
 
 // By one warp: v[0] = a lower bound of the k-th largest (k <= 256) of the 256
 // order codes v, its upper 16 bits (all of a bf16's code).  Eight codes a lane,
-// bisected.
+// two bits a step.
 __device__ __forceinline__ void kth_of_256(uint32_t* v, int k, int lane) {
   uint32_t c[8], kth = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) c[i] = v[i * 32 + lane];
 #pragma unroll 1
-  for (int bit = 31; bit >= 16; --bit) {
-    const uint32_t t = kth | (1u << bit);
-    int n = 0;
+  for (int bit = 30; bit >= 16; bit -= 2) {  // two bits a step: three counts, of at most 256 each, in one sum
+    uint32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) n += c[i] >= t;
-    if (__reduce_add_sync(0xffffffffu, n) >= k) kth = t;
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (uint32_t d = 1; d < 4; ++d) n += c[i] >= (kth | d << bit) ? 1u << (10 * (d - 1)) : 0u;
+    n = __reduce_add_sync(0xffffffffu, n);
+    uint32_t most = 0;
+#pragma unroll
+    for (uint32_t d = 1; d < 4; ++d)
+      if ((int)(n >> (10 * (d - 1)) & 1023) >= k) most = d;
+    kth |= most << bit;
   }
   if (lane == 0) v[0] = kth;
 }
@@ -492,7 +498,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
   __shared__ double base[kBeamMaxBeams];  // score - log-sum of each live beam
   __shared__ int kind[kBeamMaxBeams];     // 0 no candidate, 1 live, 2 finished
   __shared__ double list_v[kMergeList];
-  __shared__ long long list_i[kMergeList];  // beam * vocab + token
+  __shared__ long long list_i[kMergeList];  // beam, token
   __shared__ uint32_t sh_max[kMergeThreads];
   __shared__ int sh_n[2][kMergeWarps];
   __shared__ int cnt;
@@ -500,164 +506,180 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
   const int b = blockIdx.x, W = a.beams, S = a.splits, k = a.n_out;
   const int per = S * k, all = W * per;  // entries of a beam, of the sequence
   const float2* cand = a.cand + (size_t)b * all;
-  grid_dep_wait();
-  grid_dep_release();
-  if (tid == 0) cnt = 0;
-  // neighbouring entries (one beam's) go to different warps; a chunk's loads are
-  // all in flight at once, the first chunk's before anything else (what a beam
-  // without candidates left in the workspace is read, not used)
-  auto place = [&](int i) { return i * kMergeThreads + lane * kMergeWarps + warp; };
-  float2 mine[kMergeMine];
-  auto fetch = [&](int from) {
-#pragma unroll
-    for (int i = 0; i < kMergeMine; ++i)
-      if (from + place(i) < all) mine[i] = cand[from + place(i)];
-  };
-  fetch(0);
-  for (int w = warp; w < W; w += kMergeWarps) {  // a warp per beam: its slices in lane order
-    const int row = b * W + w;
-    const float2* st = a.stat + (size_t)row * S;
-    const float2 first = lane < S ? st[lane] : make_float2(kNegInf, 0.f);
-    const float sc = a.scores[row];
-    int kd = fabsf(sc) <= FLT_MAX ? (a.fin && a.fin[row] ? 2 : 1) : 0;
-    double lse = 0;
-    if (kd == 1) {
-      float M = first.x;
-      for (int s = lane + 32; s < S; s += 32) M = fmaxf(M, st[s].x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      if (M > kNegInf) {
-        // a slice's sum from its own max to the row's
-        auto term = [&](const float2& v) { return v.x > kNegInf ? (double)(v.y * rescale(v.x, M)) : 0.; };
-        double t = term(first);
-        for (int s = lane + 32; s < S; s += 32) t += term(st[s]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        lse = log_sum(M, t);
-      } else {
-        kd = 0;  // every token masked
-      }
-    }
-    if (lane == 0) {
-      kind[w] = kd;
-      base[w] = (double)sc - lse;
-    }
-  }
-  __syncthreads();
-  // cuts the list to what reaches the upper 16 bits of its k-th value's code, or,
-  // if ties leave too many, to its k best
-  auto cut = [&](int n) {
-    constexpr int kMine = (kMergeList + kMergeThreads - 1) / kMergeThreads;
-    double v[kMine];
-    long long id[kMine];
-    uint32_t c[kMine], kth = 0;
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int i = tid + j * kMergeThreads;
-      v[j] = i < n ? list_v[i] : -INFINITY;
-      id[j] = i < n ? list_i[i] : 0;
-      c[j] = i < n ? order_code(__double2float_rd(v[j])) : 0;
-    }
+  // Twice: first on one made-up candidate, nothing read or written, while the
+  // kernel before still runs, which brings in the instructions (0.2 to 0.5 us).
 #pragma unroll 1
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t t = kth | (1u << bit);
-      int m = 0;
-#pragma unroll
-      for (int j = 0; j < kMine; ++j) m += c[j] >= t;
-      m = __reduce_add_sync(0xffffffffu, m);
-      if (lane == 0) sh_n[bit & 1][warp] = m;
-      __syncthreads();
-      m = 0;
-#pragma unroll
-      for (int w = 0; w < kMergeWarps; ++w) m += sh_n[bit & 1][w];
-      if (m >= k) kth = t;
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool real = pass == 1;
+    if (real) {
+      grid_dep_wait();
+      grid_dep_release();
     }
     if (tid == 0) cnt = 0;
-    __syncthreads();
+    // neighbouring entries (one beam's) go to different warps; a chunk's loads are
+    // all in flight at once, the first chunk's before anything else (what a beam
+    // without candidates left in the workspace is read, not used)
+    auto place = [&](int i) { return i * kMergeThreads + lane * kMergeWarps + warp; };
+    float2 mine[kMergeMine];
+    auto fetch = [&](int from) {
 #pragma unroll
-    for (int j = 0; j < kMine; ++j)
-      if (c[j] >= kth && c[j] > 0) {
-        const int at = atomicAdd(&cnt, 1);
-        list_v[at] = v[j], list_i[at] = id[j];
+      for (int i = 0; i < kMergeMine; ++i) {
+        if (!real) mine[i] = make_float2(tid + i ? kNegInf : 0.f, 0.f);
+        if (real && from + place(i) < all) mine[i] = cand[from + place(i)];
       }
-    __syncthreads();
-    n = cnt;
-    if (n <= kMergeKept) return;
-    int rank[kMine];
+    };
+    fetch(0);
+    const int slices = real ? S : 0;
+    const int beams = real ? W : min(W, kMergeWarps);
+    for (int w = warp; w < beams; w += kMergeWarps) {  // a warp per beam: its slices in lane order
+      const int row = b * W + w;
+      const float2* st = a.stat + (size_t)row * S;
+      float2 first = lane < slices ? st[lane] : make_float2(kNegInf, 0.f);
+      if (!real && lane == 0) first = make_float2(0.f, 1.f);
+      const float sc = real ? a.scores[row] : 0.f;
+      int kd = fabsf(sc) <= FLT_MAX ? (real && a.fin && a.fin[row] ? 2 : 1) : 0;
+      double lse = 0;
+      if (kd == 1) {
+        float M = first.x;
+        for (int s = lane + 32; s < slices; s += 32) M = fmaxf(M, st[s].x);
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int i = tid + j * kMergeThreads;
-      rank[j] = k;
-      if (i < n) {
-        v[j] = list_v[i], id[j] = list_i[i], rank[j] = 0;
-        for (int q = 0; q < n; ++q) rank[j] += list_v[q] > v[j] || (list_v[q] == v[j] && list_i[q] < id[j]);
-      }
-    }
-    __syncthreads();
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        if (M > kNegInf) {
+          // a slice's sum from its own max to the row's
+          auto term = [&](const float2& v) { return v.x > kNegInf ? (double)(v.y * rescale(v.x, M)) : 0.; };
+          double t = term(first);
+          for (int s = lane + 32; s < slices; s += 32) t += term(st[s]);
 #pragma unroll
-    for (int j = 0; j < kMine; ++j)
-      if (rank[j] < k) list_v[rank[j]] = v[j], list_i[rank[j]] = id[j];
-    if (tid == 0) cnt = k;
-    __syncthreads();
-  };
-  double bound = -INFINITY;
-  for (int from = 0; from < all; from += kMergeChunk) {
-    double val[kMergeMine], m = -INFINITY;
-    long long pos[kMergeMine];
-#pragma unroll
-    for (int i = 0; i < kMergeMine; ++i) {
-      val[i] = -INFINITY, pos[i] = 0;
-      const int e = from + place(i);
-      if (e < all) {
-        const int w = e / per;
-        if (kind[w] == 1) {
-          if (mine[i].x > kNegInf)
-            val[i] = base[w] + (double)mine[i].x, pos[i] = (long long)w * a.vocab + __float_as_int(mine[i].y);
-        } else if (kind[w] == 2 && e == w * per) {
-          val[i] = base[w], pos[i] = (long long)w * a.vocab + a.eos;
+          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+          lse = log_sum(M, t);
+        } else {
+          kd = 0;  // every token masked
         }
       }
-      m = fmax(m, val[i]);
-    }
-    if (from + kMergeChunk < all) fetch(from + kMergeChunk);
-    if (all > kMergeFew) {  // the k-th largest of the threads' maxima: at least k entries reach it
-      sh_max[tid] = order_code(__double2float_rd(m));
-      __syncthreads();
-      if (warp == 0) kth_of_256(sh_max, k, lane);
-      __syncthreads();
-      if (sh_max[0] > order_code(kNegInf)) bound = fmax(bound, (double)from_code(sh_max[0]));
-    }
-#pragma unroll
-    for (int i = 0; i < kMergeMine; ++i)
-      if (val[i] >= bound && val[i] > -INFINITY) {
-        const int at = atomicAdd(&cnt, 1);
-        list_v[at] = val[i], list_i[at] = pos[i];
+      if (lane == 0) {
+        kind[w] = kd;
+        base[w] = (double)sc - lse;
       }
-    __syncthreads();
-    const int n = cnt;
-    __syncthreads();
-    if (n > 2 * kMergeFew && n > k) cut(n);  // so no more than kMergeKept stay
-  }
-  const int n = cnt;
-  for (int i = tid; i < n; i += kMergeThreads) {
-    const double v = list_v[i];
-    const long long id = list_i[i];
-    int rank = 0;
-    for (int q = 0; q < n; ++q) rank += list_v[q] > v || (list_v[q] == v && list_i[q] < id);
-    if (rank < k) {
-      const int w = (int)(id / a.vocab), t = (int)(id % a.vocab), at = b * k + rank;
-      a.parent[at] = w;
-      a.token[at] = t;
-      a.out[at] = (float)v;
-      if (a.fin_out) a.fin_out[at] = kind[w] == 2 || t == a.eos;
     }
-  }
-  for (int i = n + tid; i < k; i += kMergeThreads) {  // fewer candidates than asked for
-    const int at = b * k + i;
-    a.parent[at] = -1;
-    a.token[at] = -1;
-    a.out[at] = kNegInf;
-    if (a.fin_out) a.fin_out[at] = 0;
+    __syncthreads();
+    // cuts the list to what reaches the upper 16 bits of its k-th value's code, or,
+    // if ties leave too many, to its k best
+    auto cut = [&](int n) {
+      constexpr int kMine = (kMergeList + kMergeThreads - 1) / kMergeThreads;
+      double v[kMine];
+      long long id[kMine];
+      uint32_t c[kMine], kth = 0;
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        const int i = tid + j * kMergeThreads;
+        v[j] = i < n ? list_v[i] : -INFINITY;
+        id[j] = i < n ? list_i[i] : 0;
+        c[j] = i < n ? order_code(__double2float_rd(v[j])) : 0;
+      }
+#pragma unroll 1
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = kth | (1u << bit);
+        int m = 0;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) m += c[j] >= t;
+        m = __reduce_add_sync(0xffffffffu, m);
+        if (lane == 0) sh_n[bit & 1][warp] = m;
+        __syncthreads();
+        m = 0;
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; ++w) m += sh_n[bit & 1][w];
+        if (m >= k) kth = t;
+      }
+      if (tid == 0) cnt = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kMine; ++j)
+        if (c[j] >= kth && c[j] > 0) {
+          const int at = atomicAdd(&cnt, 1);
+          list_v[at] = v[j], list_i[at] = id[j];
+        }
+      __syncthreads();
+      n = cnt;
+      if (n <= kMergeKept) return;
+      int rank[kMine];
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        const int i = tid + j * kMergeThreads;
+        rank[j] = k;
+        if (i < n) {
+          v[j] = list_v[i], id[j] = list_i[i], rank[j] = 0;
+          for (int q = 0; q < n; ++q) rank[j] += list_v[q] > v[j] || (list_v[q] == v[j] && list_i[q] < id[j]);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kMine; ++j)
+        if (rank[j] < k) list_v[rank[j]] = v[j], list_i[rank[j]] = id[j];
+      if (tid == 0) cnt = k;
+      __syncthreads();
+    };
+    double bound = -INFINITY;
+    for (int from = 0; from < (real ? all : 1); from += kMergeChunk) {
+      double val[kMergeMine], m = -INFINITY;
+      long long pos[kMergeMine];
+#pragma unroll
+      for (int i = 0; i < kMergeMine; ++i) {
+        val[i] = -INFINITY, pos[i] = 0;
+        const int e = from + place(i);
+        if (from + i * kMergeThreads < all && e < all) {  // the first for the whole CTA
+          const int w = e / per;
+          if (kind[w] == 1) {
+            if (mine[i].x > kNegInf)
+              val[i] = base[w] + (double)mine[i].x, pos[i] = (long long)w << 32 | __float_as_int(mine[i].y);
+          } else if (kind[w] == 2 && e == w * per) {
+            val[i] = base[w], pos[i] = (long long)w << 32 | a.eos;
+          }
+        }
+        m = fmax(m, val[i]);
+      }
+      if (real && from + kMergeChunk < all) fetch(from + kMergeChunk);
+      if (all > kMergeFew) {  // the k-th largest of the threads' maxima: at least k entries reach it
+        sh_max[tid] = order_code(__double2float_rd(m));
+        __syncthreads();
+        if (warp == 0) kth_of_256(sh_max, k, lane);
+        __syncthreads();
+        if (sh_max[0] > order_code(kNegInf)) bound = fmax(bound, (double)from_code(sh_max[0]));
+      }
+#pragma unroll
+      for (int i = 0; i < kMergeMine; ++i)
+        if (val[i] >= bound && val[i] > -INFINITY) {
+          const int at = atomicAdd(&cnt, 1);
+          list_v[at] = val[i], list_i[at] = pos[i];
+        }
+      __syncthreads();
+      const int n = cnt;
+      __syncthreads();
+      if (n > 2 * kMergeFew && n > k) cut(n);  // so no more than kMergeKept stay
+    }
+    const int n = cnt;
+    for (int i = tid >> 3; i < (n + 3 & ~3); i += kMergeThreads / 8) {  // eight threads an entry
+      const double v = i < n ? list_v[i] : -INFINITY;
+      const long long id = i < n ? list_i[i] : 0;
+      int rank = 0;
+      for (int q = tid & 7; q < n; q += 8) rank += list_v[q] > v || (list_v[q] == v && list_i[q] < id);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      if (i < n && rank < k && real && (tid & 7) == 0) {
+        const int w = (int)(id >> 32), t = (int)id, at = b * k + rank;
+        a.parent[at] = w;
+        a.token[at] = t;
+        a.out[at] = (float)v;
+        if (a.fin_out) a.fin_out[at] = kind[w] == 2 || t == a.eos;
+      }
+    }
+    for (int i = real ? n + tid : k; i < k; i += kMergeThreads) {  // fewer candidates than asked for
+      const int at = b * k + i;
+      a.parent[at] = -1;
+      a.token[at] = -1;
+      a.out[at] = kNegInf;
+      if (a.fin_out) a.fin_out[at] = 0;
+    }
+    __syncthreads();
   }
 }
 
@@ -667,13 +689,15 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
 // number that makes rounds of resident CTAs x (tiles a warp walks + what a CTA
 // costs besides, about five tiles) the smallest.
 int beam_splits(int batch, int beams, int vocab, int f32) {
-  const long long rows = (long long)batch * beams, tiles = (vocab + (f32 ? 511 : 1023)) / (f32 ? 512 : 1024);
-  const long long resident = 148 * 4, most = std::min<long long>(std::max<long long>(1, tiles / kRowWarps), 2 * resident);
-  long long best = 1, cost = -1;
-  for (long long s = 1; s <= most; ++s) {
-    const long long per = (tiles + s * kRowWarps - 1) / (s * kRowWarps);
-    const long long c = (rows * s + resident - 1) / resident * (per + 5);
-    if (cost < 0 || c < cost) best = s, cost = c;
+  const unsigned rows = (unsigned)(batch * beams), tiles = ((unsigned)vocab + (f32 ? 511 : 1023)) / (f32 ? 512 : 1024);
+  constexpr unsigned resident = 148 * 4;
+  const unsigned most = std::min(std::max(1u, tiles / kRowWarps), 2 * resident);
+  unsigned best = 1;
+  unsigned long long cost = ~0ull;
+  for (unsigned s = 1; s <= most; ++s) {
+    const unsigned per = (tiles + s * kRowWarps - 1) / (s * kRowWarps);
+    const unsigned long long c = ((unsigned long long)rows * s + resident - 1) / resident * (per + 5);
+    if (c < cost) best = s, cost = c;
   }
   return (int)best;
 }

@@ -475,11 +475,16 @@ static llmoc_status check_beam(const llmoc_beam_desc* d, const char* who) {
   return LLMOC_OK;
 }
 
-size_t llmoc_beam_workspace_bytes(const llmoc_beam_desc* d) {
-  if (check_beam(d, "llmoc_beam_workspace_bytes") != LLMOC_OK) return 0;
-  const int splits = std::max(beam_splits(d->batch, d->beams, d->vocab, 0), beam_splits(d->batch, d->beams, d->vocab, 1));
-  const size_t lists = (size_t)d->batch * d->beams * splits;
+// the workspace of a checked description; splits: slices per row of bf16 and of fp32 logits
+static size_t beam_bytes(const llmoc_beam_desc* d, int (&splits)[2]) {
+  for (int f32 = 0; f32 < 2; ++f32) splits[f32] = beam_splits(d->batch, d->beams, d->vocab, f32);
+  const size_t lists = (size_t)d->batch * d->beams * std::max(splits[0], splits[1]);
   return up256(lists * d->n_out * 8) + up256(lists * 8);
+}
+
+size_t llmoc_beam_workspace_bytes(const llmoc_beam_desc* d) {
+  int splits[2];
+  return check_beam(d, "llmoc_beam_workspace_bytes") == LLMOC_OK ? beam_bytes(d, splits) : 0;
 }
 
 llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int64_t ld, int logits_dtype,
@@ -513,11 +518,12 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
     for (int i = 0; i < o; ++i)
       if (overlap(outs[o], outs[i])) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": two outputs overlap");
   }
-  if (!workspace || workspace_bytes < llmoc_beam_workspace_bytes(d))
+  int splits[2];
+  const size_t need = beam_bytes(d, splits);
+  if (!workspace || workspace_bytes < need)
     return refuse(LLMOC_ERR_WORKSPACE, std::string(who) + ": workspace too small");
   if (!aligned(workspace, 8)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace is not aligned to 8");
-  const long long used = (long long)llmoc_beam_workspace_bytes(d);
-  const Rows wr{workspace, used, used, 1};
+  const Rows wr{workspace, (long long)need, (long long)need, 1};
   for (const Rows& r : in)
     if (overlap(wr, r)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace overlaps an input");
   for (const Rows& r : outs)
@@ -539,7 +545,7 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
   a.token = token;
   a.out = out_scores;
   a.fin_out = finished_out;
-  a.splits = beam_splits(d->batch, d->beams, d->vocab, a.f32);
+  a.splits = splits[a.f32];
   a.vec = vec_rows(logits, ld * (long long)es);
   const size_t lists = (size_t)rows * a.splits;
   a.cand = (float2*)workspace;
