@@ -47,6 +47,7 @@
 // 16-byte load per 32 k and 8 tokens, with the group sums beside them.  One
 // token is stored once and read as all eight columns.
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "ops.cuh"
@@ -348,7 +349,7 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
   int ksw = 1, c = 1;
   auto fits = [&](int w, int k) {
     const int rbt = kLinWarps / w;
-    return (long long)((a.mt + rbt - 1) / rbt) * ntb * k <= 148 && a.nb >= w * k;
+    return (long long)((a.mt + rbt - 1) / rbt) * ntb * k <= cluster_ctas(k) && a.nb >= w * k;
   };
   while (ksw < kLinWarps && TP * ksw * 2 <= 16 && fits(2 * ksw, c)) ksw *= 2, ++p.lk;
   while (c < 8 && fits(ksw, 2 * c)) c *= 2, ++p.lc;
@@ -438,6 +439,37 @@ __global__ void k_lin_pack(const LinPack a) {
 }
 
 }  // namespace
+
+int cluster_ctas(int c) {
+  static std::atomic<int> known[64][9];  // by device; 0: not asked yet
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& at = known[dev & 63][c];
+  int n = dev < 64 ? at.load(std::memory_order_relaxed) : 0;
+  if (n) return n;
+  const auto kernel = k_linear<4, true, 1, 1>;  // any kernel with one CTA an SM
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)c);
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = kLinSmemMax;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (c == 1) {
+    n = 148;
+  } else if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmemMax) != cudaSuccess ||
+             cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 100 / c * c;  // what any device has
+  } else {
+    n *= c;
+  }
+  if (dev < 64) at.store(n, std::memory_order_relaxed);
+  return n;
+}
 
 cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st) {
   k_lin_pack<<<148 * 8, 256, 0, st>>>(a);

@@ -685,11 +685,11 @@ cudaError_t launch_u(const LinArgs& a, cudaStream_t st) {
   p.steps = (a.K + 127) / 128;
   const long long units = (long long)((a.mt + 7) / 8) * ntb;
   // CTAs per cluster: the fewest rounds x (steps + what a CTA costs besides,
-  // about ten steps); a cluster's CTAs share a GPC, which leaves some SMs over
-  static const int resident[9] = {0, 148, 148, 138, 136, 130, 126, 126, 128};
+  // about ten steps)
   long long cost = -1;
   for (int c = 1; c <= 8 && c <= p.steps; ++c) {
-    const long long now = (units * c + resident[c] - 1) / resident[c] * ((p.steps + c - 1) / c + 10);
+    const int at_once = cluster_ctas(c);
+    const long long now = (units * c + at_once - 1) / at_once * ((p.steps + c - 1) / c + 10);
     if (cost < 0 || now < cost) cost = now, p.c = c;
   }
   const int smem = UCfg<FL, AWQ>::smem(p.N);

@@ -41,6 +41,9 @@ struct LinPack {
 };
 cudaError_t launch_lin_pack(const LinPack& a, cudaStream_t st);
 cudaError_t launch_linear(const LinArgs& a, int fl, bool awq, cudaStream_t st);
+// CTAs of c-wide clusters that are resident at once on the current device, one on
+// an SM (a cluster stays within a GPC, whose SMs are rarely a multiple of c)
+int cluster_ctas(int c);
 // linear_umma.cu: the same product for tens of tokens (tcgen05); zp < 16
 cudaError_t launch_linear_umma(const LinArgs& a, int fl, bool awq, cudaStream_t st);
 
