@@ -79,9 +79,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// *p of the cluster's CTA `rank` (c = 1: of this CTA)
-__device__ __forceinline__ float ld_cluster(const float* p, int rank, int c) {
-  if (c == 1) return *p;
+// *p of the cluster's CTA `rank`
+__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
   uint32_t at;
   float v;
   const uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -298,26 +297,41 @@ __global__ void __launch_bounds__(kLinThreads, 1) k_linear(const LinArgs a, cons
           for (int i = 0; i < 4; ++i)
             store(((unit << lr) + wt) * 16 + g + (i >> 1) * 8, tok0 + n * 8 + 2 * t + (i & 1), acc[n][i]);
       } else {
-        // partial sums of the K slices, added in slice order (rank, then warp);
-        // such a grid has a cluster per unit, so the buffer is written once
+        // partial sums of the K slices, added in slice order (warps, then ranks); such
+        // a grid has a cluster per unit, so the buffer is written once
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             red[(warp * kCols + n * 8 + 2 * t + (i & 1)) * kColLd + g + (i >> 1) * 8] = acc[n][i];
-        if (c > 1)
-          cluster_sync();
-        else
-          __syncthreads();
-        const int lrows = lr + 4, step = kLinThreads << p.lc;
+        __syncthreads();
+        const int lrows = lr + 4;
         const int cols = min(kCols, a.T - tok0);
-        for (int e = threadIdx.x + rank * kLinThreads; e < cols << lrows; e += step) {
-          const int row = e & ((1 << lrows) - 1), col = e >> lrows, w0 = row >> 4;
-          const float* at = red + (w0 * kCols + col) * kColLd + (row & 15);
+        auto at = [&](int e) {  // the sum of the first warp of row e's tile
+          const int row = e & ((1 << lrows) - 1), col = e >> lrows;
+          return red + ((row >> 4) * kCols + col) * kColLd + (row & 15);
+        };
+        for (int e = threadIdx.x; e < cols << lrows; e += kLinThreads) {
+          float* p0 = at(e);
           float v = 0.f;
-          for (int q = 0; q < c; ++q)
-            for (int s = 0; s < ksw; ++s) v += ld_cluster(at + (s << lr) * kCols * kColLd, q, c);
-          store((unit << lrows) + row, tok0 + col, v);
+          for (int s = 0; s < ksw; ++s) v += p0[(s << lr) * kCols * kColLd];
+          if (c > 1)
+            *p0 = v;
+          else
+            store((unit << lrows) + (e & ((1 << lrows) - 1)), tok0 + (e >> lrows), v);
+        }
+        if (c > 1) {
+          cluster_sync();
+          for (int e = threadIdx.x + rank * kLinThreads; e < cols << lrows; e += kLinThreads << p.lc) {
+            const float* p0 = at(e);
+            float w[8];  // the ranks' sums, all on their way at once
+#pragma unroll
+            for (int q = 0; q < 8; ++q) w[q] = q < c ? ld_cluster(p0, q) : 0.f;
+            float v = 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v += w[q];
+            store((unit << lrows) + (e & ((1 << lrows) - 1)), tok0 + (e >> lrows), v);
+          }
         }
       }
 #pragma unroll
