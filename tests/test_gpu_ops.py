@@ -973,3 +973,18 @@ def test_norm_many_rows(H, T, rdt):
     wr, er, wn, en = ref_norm(b, r, None, c)
     check_rows(ro, wr, er, "residual")
     check_rows(no, wn, en, "norm")
+
+
+@pytest.mark.parametrize("B,W", [(40, 8), (3, 100), (128, 8), (129, 8), (1000, 1)])
+@pytest.mark.parametrize("share", [0.0, 0.3, 0.95, 1.0])
+def test_select_many_rows_some_finished(B, W, share):
+    """Finished beams and beams without a score among many: the others' rows
+    keep their places."""
+    V, k = 1500, min(W, 5)
+    g = gen(B + W)
+    logits = torch.randn((B * W, V), generator=g, device="cuda")
+    scores = torch.randn((B, W), generator=g, device="cuda")
+    scores[torch.rand((B, W), generator=g, device="cuda") < 0.2] = float("-inf")
+    scores[0, 0] = float("nan")
+    fin = (torch.rand((B, W), generator=g, device="cuda") < share).to(torch.uint8)
+    check_select(logits, scores, fin, 3, k)
