@@ -24,11 +24,12 @@
 //                 a bound, what reaches it, ranked by counting.
 //
 // What bounds it (graph replay): 32 sequences x 8 beams x 248320 bf16 logits take
-// 46.4 us, 2.7 TB/s; of those the exponentials alone, 4 a clock and scheduler, are
+// 44.4 us, 2.9 TB/s; of those the exponentials alone, 4 a clock and scheduler, are
 // 14 us, and with the unpacking, sums and comparisons a scheduler needs some 360
-// cycles for a warp's 1024 elements.  Rows copied ahead in bulk took 48.3 us: it
-// does not wait for memory.  8 x 4 x 131072 fp32 with 8 candidates take 15.5 us
-// (1.1 TB/s), 1 x 4 x 32003 8.4 us, of which the two launches and a chain of load,
+// cycles for a warp's 1024 elements.  Rows copied ahead in bulk were 3 % slower: it
+// does not wait for memory.  Nor does it gain from CTAs gathered on the live rows
+// when some are finished.  8 x 4 x 131072 fp32 with 8 candidates take 15.0 us
+// (1.1 TB/s), 1 x 4 x 32003 7.6 us, of which the two launches and a chain of load,
 // first bound, list and merge are nearly all; the merge has 3 to 5 us of each.
 //
 // Order of summation is fixed by the slice and thread numbers alone, so equal
@@ -52,6 +53,7 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kListMax = 512;
+constexpr int kFewHits = 6;   // lanes of a tile whose elements are looked at one lane after the other
 constexpr int kListCut = 64;  // list length above which the closing bound is applied once more
 constexpr float kNegInf = -INFINITY;
 
@@ -380,7 +382,30 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
       // give both sides a copy of the sums, one after the other (measured: 1.7
       // times the exponentials)
       const bool hit = tm >= bound && tm > kNegInf && tm <= FLT_MAX;
-      if (__any_sync(0xffffffffu, hit)) {
+      unsigned hits = __ballot_sync(0xffffffffu, hit);
+      if (__popc(hits) <= kFewHits) {
+        // lane by lane, the warp looks at the lane's elements, one a thread: 0.1 us
+        // where walking through them took 1.5 (32 x 8 x 248320: 46.5 -> 44.4 us)
+        while (hits) {
+          const int from = __ffs(hits) - 1;
+          hits &= hits - 1;
+          uint32_t w = 0;
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              const uint32_t x = __shfl_sync(0xffffffffu, u[q][i], from);
+              if (q * kWords + i == (F32 ? lane : lane >> 1)) w = x;
+            }
+          const float v = __uint_as_float(F32 || (lane & 1) ? (F32 ? w : w & 0xFFFF0000u) : w << 16);
+          const bool in = lane < N && v >= bound && v > kNegInf;
+          const unsigned all = __ballot_sync(0xffffffffu, in);
+          int at = 0;
+          if (lane == 0 && all) at = atomicAdd(&sh_cnt, __popc(all));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
+          if (in && at < kListMax) list_v[at] = v, list_i[at] = t * kTile + ((lane >> 3) * 32 + from) * 8 + (lane & 7);
+        }
+      } else {
 #pragma unroll 1
         for (int q = 0; q < Q; ++q) {
           uint32_t w[kWords];  // u[q]
