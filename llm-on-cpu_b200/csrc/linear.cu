@@ -9,8 +9,8 @@
 // Weights are packed for this kernel (k_lin_pack): per 16-row tile a stream of
 // blocks of 256 k, each four 512-byte chunks of words (64 k: lane (g, t)'s 16
 // bytes at 64 g + 16 (t xor g / 2), two words of row g, then two of row g + 8, a
-// word the 8 k from 8 t of one of the chunk's two 32 k) followed by the block's scales (and zeros) as fp16 pairs of rows
-// (g, g + 8).  Groups that are other multiples of 32, 64 or 128 repeat their
+// word the 8 k from 8 t of one of the chunk's two 32 k), then the block's scales
+// (and zeros) as fp16 pairs of rows (g, g + 8).  Groups that are other multiples of 32, 64 or 128 repeat their
 // scale, so a block holds 8, 4 or 2 groups of 32, 64 or 128.
 //
 // Work.  A warp owns a tile against NT * 8 tokens over a slice of K.  The
