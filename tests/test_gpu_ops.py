@@ -988,3 +988,54 @@ def test_select_many_rows_some_finished(B, W, share):
     scores[0, 0] = float("nan")
     fin = (torch.rand((B, W), generator=g, device="cuda") < share).to(torch.uint8)
     check_select(logits, scores, fin, 3, k)
+
+
+FIRST_CALL = """
+import sys
+import torch
+import llmoc_b200 as L
+T, M, K, gs = (int(v) for v in sys.argv[1:5])
+q = torch.randint(0, 256, (M, K // 2), device="cuda", dtype=torch.uint8)
+s = torch.rand((M, K // gs), device="cuda").half()
+torch.cuda.synchronize()
+lin = L.Int4Linear.create([L.view(q, s, None, M, K, gs, L.SCHEME_AWQ_SYM, 7)], on_device=True)
+x, y = torch.randn((T, K), device="cuda").to(torch.bfloat16), torch.zeros((T, M), device="cuda")
+r, n = torch.randn((T, K), device="cuda").to(torch.bfloat16), torch.zeros((T, K), device="cuda", dtype=torch.bfloat16)
+norm = L.ResidualNorm(K, pre="rms")
+bs = L.BeamSearch(1, T, M, T)
+ws = torch.empty(bs.workspace_bytes(), device="cuda", dtype=torch.uint8)
+sc, pa = torch.zeros((1, T), device="cuda"), torch.zeros((1, T), device="cuda", dtype=torch.int32)
+out = [pa, pa.clone(), sc.clone()]
+ro = L.BeamReorder([y.view(1, T, M)], [y.clone().view(1, T, M)], 1, T, T)
+st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+def step(stream):
+    norm.forward(T, x, r, None, n, stream=stream)
+    lin.forward(x, T, y, stream=stream)
+    bs.select(y, sc, *out, ws, ws.numel(), stream=stream)
+    ro.run(out[0], stream=stream)
+with torch.cuda.graph(graph, stream=st):
+    step(torch.cuda.current_stream())
+graph.replay()
+torch.cuda.synchronize()
+got = [v.clone() for v in (n, y, *out, ro._keep[1][0])]
+for v in (n, y, *out, ro._keep[1][0]):
+    v.zero_()
+step(torch.cuda.current_stream())
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (n, y, *out, ro._keep[1][0])))
+lin.status(torch.cuda.current_stream())
+"""
+
+
+@pytest.mark.parametrize("T,M,K,gs", [(1, 512, 1024, 128), (8, 512, 4096, 32), (40, 2048, 4096, 64)])
+def test_first_calls_of_a_process_are_captured(T, M, K, gs):
+    """Nothing a first call sets up keeps it out of a capture."""
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(os.path.abspath(L.__file__)),
+                                                       os.environ.get("PYTHONPATH", "")]))
+    p = subprocess.run([sys.executable, "-c", FIRST_CALL, *map(str, (T, M, K, gs))], env=env, capture_output=True,
+                       text=True, timeout=300)
+    assert p.returncode == 0, p.stderr[-2000:]
