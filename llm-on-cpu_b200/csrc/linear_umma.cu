@@ -48,9 +48,21 @@
 // gives up sets the handle's error word (llmoc_int4_linear_status) and every role
 // drains and exits.
 //
-// Why the parity waits are sound: each barrier's waiter waits for every phase of
-// it in order and is at most one phase ahead of it: a dequantising or drain warp
-// waits for each weight block, also for a first one of which it needs no step.
+// Why the parity waits are sound.  A waiter looks at every phase of a barrier before
+// the next can complete, and an arrival comes after the phase before is complete.
+// The rings of the weights, activations and accumulators give both, as a slot and
+// its barriers turn together (a dequantising or drain warp waits for each weight
+// block, also for a first one of which it needs no step).  `full` and `empty` do
+// not belong to a slot but turn by steps, kSteps of them, since all that holds the
+// four warps of a group and the two groups of dequantisers together is the wait for
+// `empty` of step j - kASlots.  With 3 A slots it says that the other group was
+// through with step j - 3, so that j - 6 is complete, and while a warp is at step j
+// the other group completes no step beyond j + 1: 6 entries.  (With 4, as many as
+// B slots, a warp could arrive for step j while one beside it had not for j - 4, and
+// the MMAs read unwritten rows; and a group late at its wait for step j - 3 missed
+// it once j + 1 was complete, which has the same parity.)  With 4 A slots it is a
+// wait for the warp's own group: a warp at step j knows that all of them are through
+// with j - 4, and so with j - 6.  tests/test_umma_waits.py walks the interleavings.
 // Sums of step j are overwritten by step j + 16's, whose activations have landed
 // only after the MMAs of step j + 10 completed; their issuer had waited until every
 // drain warp gave back step j + 6's accumulator, which each does after it is
@@ -81,6 +93,7 @@ struct UCfg {
   static constexpr int kASlots = kSplit ? 3 : 4;     // A slots
   static constexpr int kACols = kSplit ? 128 : 64;   // TMEM columns of one
   static constexpr int kXSlots = kZCols ? 4 : 6;     // B slots
+  static constexpr int kSteps = 6;                   // entries of the barrier rings `full` and `empty`
   static constexpr int kRing = kZCols ? 3 : 6;       // blocks of weights, two steps each
   static constexpr int kBB = lin_block_bytes(FL, !AWQ);
   static constexpr int kParts = kZCols ? 3 : 2;      // 64-wide parts of a B slot
@@ -88,6 +101,7 @@ struct UCfg {
   static constexpr int smem(int n) { return 1024 + kXSlots * kParts * n * 128 + kSideBytes + kRing * 8 * kBB; }
   static_assert(kAcc * 64 + kASlots * kACols <= 512, "TMEM");
   static_assert(smem(kUCols) <= 226 * 1024, "shared memory");
+  static_assert(kXSlots <= kSteps && kSteps == 6 && (kASlots == 3 || kASlots == 4), "the turns argued above");
 };
 
 struct UPlan {
@@ -229,10 +243,11 @@ __global__ void __launch_bounds__(kULinThreads, 1)
     k_lin_umma(const LinArgs a, const UPlan p, const __grid_constant__ CUtensorMap xmap) {
   using C = UCfg<FL, AWQ>;
   constexpr bool kSplit = C::kSplit, kSums = C::kSums, kZCols = C::kZCols;
-  constexpr int kGs = C::kGs, kBB = C::kBB, kAcc = C::kAcc, kASlots = C::kASlots, kXSlots = C::kXSlots, kRing = C::kRing;
+  constexpr int kGs = C::kGs, kBB = C::kBB, kAcc = C::kAcc, kASlots = C::kASlots, kXSlots = C::kXSlots, kRing = C::kRing,
+                kSteps = C::kSteps;
   constexpr int kGrp = 8 / FL;  // groups per block of the stream
   extern __shared__ __align__(1024) unsigned char usm[];
-  __shared__ __align__(8) uint64_t xFull[kXSlots], full[kXSlots], empty[kXSlots], wFull[kRing], wEmpty[kRing], accFull[4],
+  __shared__ __align__(8) uint64_t xFull[kXSlots], full[kSteps], empty[kSteps], wFull[kRing], wEmpty[kRing], accFull[4],
       accEmpty[4], done[4];
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
@@ -255,8 +270,8 @@ __global__ void __launch_bounds__(kULinThreads, 1)
   auto drained = [&](int j) { return !kSplit || (j / kAcc + j) % C::kHold == 0 || j + kAcc >= n; };
   const int halves = p.N > 16 ? 2 : 1;  // drain warps per quadrant with columns
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kXSlots; ++s) {
-      mb_init(&xFull[s], 1);
+    for (int s = 0; s < kXSlots; ++s) mb_init(&xFull[s], 1);
+    for (int s = 0; s < kSteps; ++s) {
       mb_init(&full[s], 4 + (p.tma && !kSums ? 0 : 2));  // four dequantising warps, the activation warps
       mb_init(&empty[s], 1);
     }
@@ -307,11 +322,12 @@ __global__ void __launch_bounds__(kULinThreads, 1)
       bool fresh = true;  // the next MMAs start a new sum
       uint32_t drains = 0;
       for (int j = warp; j < n; j += kAcc) {
-        const int slot = j % kXSlots, use = j / kXSlots & 1;
+        const int slot = j % kXSlots, step = j % kSteps;
         const uint32_t ta = tmem + kAcc * 64 + j % kASlots * C::kACols;
         const uint64_t dB = dB0 + slot * (slot_bytes >> 4);
         // the step's operands, and the accumulator's last sum drained
-        if ((p.tma && !kSums && !mb_wait(&xFull[slot], use, &abort_flag)) || !mb_wait(&full[slot], use, &abort_flag) ||
+        if ((p.tma && !kSums && !mb_wait(&xFull[slot], j / kXSlots & 1, &abort_flag)) ||
+            !mb_wait(&full[step], j / kSteps & 1, &abort_flag) ||
             (fresh && drains && !mb_wait(&accEmpty[warp], (drains - 1) & 1, &abort_flag))) {
           ok = false;
           break;
@@ -329,7 +345,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
           umma_commit(&accFull[warp]);
           ++drains;
         }
-        umma_commit(&empty[slot]);
+        umma_commit(&empty[step]);
       }
       // every MMA this thread issued has completed once its `done` fires
       umma_commit(&done[warp]);
@@ -346,7 +362,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
       int j = 0;
       for (; j < n; ++j) {
         const int slot = j % kXSlots;
-        if (j >= kXSlots && !mb_wait(&empty[slot], (j / kXSlots - 1) & 1, &abort_flag)) {
+        if (j >= kXSlots && !mb_wait(&empty[(j - kXSlots) % kSteps], (j - kXSlots) / kSteps & 1, &abort_flag)) {
           ok = false;
           break;
         }
@@ -427,7 +443,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
         if (p.tma) {
           ok = warp_wait(&xFull[slot], j / kXSlots & 1);
         } else {
-          ok = j < kXSlots || warp_wait(&empty[slot], (j / kXSlots - 1) & 1);
+          ok = j < kXSlots || warp_wait(&empty[(j - kXSlots) % kSteps], (j - kXSlots) / kSteps & 1);
           const int k = (j0 + j) * 128 + pc * 8;
           for (int i = lane >> 4; ok && i < 32 && 32 * aw + i < p.N; i += 2) {
             const int r = 32 * aw + i;
@@ -449,7 +465,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
         if (kSums && 32 * aw < p.N) sums(j);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mb_arrive(&full[slot]);
+        if (lane == 0) mb_arrive(&full[j % kSteps]);
       }
   } else if (warp < 16) {
     // the words of this thread's row: 8 bytes of each 16 of its pair of rows' 64 in
@@ -468,7 +484,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
       const int bi = ((j0 + j) >> 1) - b0, slot = bi % kRing, odd = (j0 + j) & 1;
       if (j >= kASlots) {  // the A slot's last MMAs
         const int o = j - kASlots;
-        if (!warp_wait(&empty[o % kXSlots], o / kXSlots & 1)) {
+        if (!warp_wait(&empty[o % kSteps], o / kSteps & 1)) {
           ok = false;
           break;
         }
@@ -537,7 +553,7 @@ __global__ void __launch_bounds__(kULinThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mb_arrive(&full[j % kXSlots]);
+        mb_arrive(&full[j % kSteps]);
         mb_arrive(&wEmpty[slot]);
       }
     }
