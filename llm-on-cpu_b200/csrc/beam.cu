@@ -69,9 +69,13 @@ __device__ __forceinline__ float from_code(uint32_t c) {
 // a before b in the order "larger value, then smaller index"
 __device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
 
-// exp(x - m) as 2^(x * kLog2e - fl(m * kLog2e)): the rounding of the constant and
+// exp(x - m) as 2^(x * kLog2e - log2_ref(m)): the rounding of the constant and
 // of the product drop out of the log-sum, which the merge corrects (log_sum).
+// Every sum and every change of reference goes by the same rounded product: an
+// unrounded one in its place (a contracted multiply-add) is off by 2^-24 of the
+// logits' own size.
 constexpr float kLog2e = 1.44269504f;
+__device__ __forceinline__ float log2_ref(float m) { return __fmul_rn(m, kLog2e); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -81,12 +85,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr float kScaleMax = 1e38f;
 // the factor from a sum relative to m to one relative to n
 __device__ __forceinline__ float rescale(float m, float n) {
-  return exp2_fast(fabsf(m) <= kScaleMax && fabsf(n) <= kScaleMax ? m * kLog2e - n * kLog2e : (m - n) * kLog2e);
+  return exp2_fast(fabsf(m) <= kScaleMax && fabsf(n) <= kScaleMax ? __fsub_rn(log2_ref(m), log2_ref(n)) : (m - n) * kLog2e);
 }
 // log sum exp of a row whose largest value is m, from that sum relative to m
 __device__ __forceinline__ double log_sum(float m, double s) {
   if (fabsf(m) > kScaleMax) return (double)m + log(s);
-  const float c = m * kLog2e;
+  const float c = log2_ref(m);
   return (double)m + log(s) + ((double)c - (double)m * (double)kLog2e) * 0.69314718055994531;
 }
 
@@ -318,7 +322,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
     return v;
   };
   float m = kNegInf;                     // this lane's max
-  float ref = kNegInf, c = 0.f, s = 0.f;  // its reference, fl(ref * kLog2e), and sum
+  float ref = kNegInf, c = 0.f, s = 0.f;  // its reference, log2_ref(ref), and sum
   float bound = kNegInf;                 // at least k elements of the slice reach it
   float shown = kNegInf;                 // the maximum published for this lane's group
   auto publish = [&]() {
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
   auto move_ref = [&](float to) {
     s = s > 0.f ? s * rescale(ref, to) : 0.f;
     ref = to;
-    c = to * kLog2e;
+    c = log2_ref(to);
   };
   auto take = [&](float v, int i) {
     const int at = atomicAdd(&sh_cnt, 1);
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
       const int i = index(t, j);
       const float v = i < a.vocab ? logit_at(a, base + i) : kNegInf;
       if (v > kNegInf) {
-        s += exp2_fast((v - ref) * kLog2e);
+        s += exp2_fast(fabsf(ref) <= kScaleMax ? fmaf(v, kLog2e, -c) : (v - ref) * kLog2e);
         if (v >= bound && !taken) take(v, i);
       }
     }

@@ -1039,3 +1039,18 @@ def test_first_calls_of_a_process_are_captured(T, M, K, gs):
     p = subprocess.run([sys.executable, "-c", FIRST_CALL, *map(str, (T, M, K, gs))], env=env, capture_output=True,
                        text=True, timeout=300)
     assert p.returncode == 0, p.stderr[-2000:]
+
+
+@pytest.mark.parametrize("V", [500, 3000, 20011, 70001])
+@pytest.mark.parametrize("offset", [1000.0, -1000.0, 100.0, -30000.0])
+@pytest.mark.parametrize("nan", [False, True])
+def test_select_with_a_common_offset(V, offset, nan):
+    """A row's log-sum does not depend on where its logits lie, nor on which of
+    its tiles hold a NaN (the tolerance is check_select's, which has no term in
+    the logits: the reference they are summed to is one and the same number)."""
+    B, W = 3, 4
+    logits = torch.randn((B * W, V), generator=gen(V), device="cuda") * 3 + offset
+    logits[1] = logits[0]
+    if nan:
+        logits[1::2, V // 3] = float("nan")
+    check_select(logits, -20 * torch.rand((B, W), generator=gen(1), device="cuda"), None, -1, 5)
