@@ -448,7 +448,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_beam_rows(const __grid_const
       }
       const float ts = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       if (tm <= FLT_MAX) m = fmaxf(m, tm);
-      if (ts <= FLT_MAX && fabsf(ref) <= kScaleMax)
+      // (a lane that has met masked logits only has no reference yet, and nothing to add)
+      if (ts <= FLT_MAX && (fabsf(ref) <= kScaleMax || tm == kNegInf))
         s += ts;
       else  // a NaN, +inf (no candidates taken yet), or products that leave fp32
         careful(t, tm <= FLT_MAX);

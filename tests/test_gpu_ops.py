@@ -1054,3 +1054,45 @@ def test_select_with_a_common_offset(V, offset, nan):
     if nan:
         logits[1::2, V // 3] = float("nan")
     check_select(logits, -20 * torch.rand((B, W), generator=gen(1), device="cuda"), None, -1, 5)
+
+
+@pytest.mark.parametrize("V", [3000, 20011, 131072])
+@pytest.mark.parametrize("keep", [0.1, 0.001])
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_select_mostly_masked(V, keep, dt):
+    """A mask that leaves few tokens, the same for all beams or one for each,
+    with NaN in some of the masked places."""
+    B, W = 4, 4
+    g = gen(V)
+    for rows in (1, B * W):
+        logits = torch.randn((B * W, V), generator=g, device="cuda").to(dt)
+        u = torch.rand((rows, V), generator=g, device="cuda")
+        logits.masked_fill_(u > keep, float("-inf"))
+        logits.masked_fill_(u > 0.9999, float("nan"))
+        check_select(logits, -20 * torch.rand((B, W), generator=g, device="cuda"), None, -1, 6)
+
+
+def test_select_mostly_masked_takes_no_longer():
+    """A lane that meets masked logits only has nothing to add and no second
+    look to take: such rows are read as fast as full ones (0.95 of their time;
+    3.6 times it when each of their tiles was read again)."""
+    B, W, V, k = 32, 8, 248320, 8
+    g = gen(9)
+    full = torch.randn((B * W, V), generator=g, device="cuda").to(BF16)
+    few = full.masked_fill(torch.rand((1, V), generator=g, device="cuda") > 0.001, float("-inf"))
+    scores = -20 * torch.rand((B, W), generator=g, device="cuda")
+    bs = L.BeamSearch(B, W, V, k)
+    ws = torch.empty(bs.workspace_bytes(), device="cuda", dtype=torch.uint8)
+    parent = torch.empty((B, k), dtype=torch.int32, device="cuda")
+    outs = (parent, parent.clone(), torch.empty((B, k), device="cuda"))
+    times = {True: [], False: []}
+    for rep in range(12):  # in turn, the first two to warm up
+        for masked in (False, True):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            for _ in range(10):
+                bs.select(few if masked else full, scores, *outs, ws, ws.numel(), stream=stream())
+            b.record()
+            b.synchronize()
+            times[masked].append(a.elapsed_time(b))
+    assert float(np.median(times[True][2:])) < 2 * float(np.median(times[False][2:]))
