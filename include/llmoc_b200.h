@@ -421,7 +421,8 @@ LLMOC_API llmoc_status llmoc_moe_forward_block(const llmoc_moe_layer* layer, con
  * finished_out[b][k] = the parent is finished, or the token is eos_token.
  * finished and finished_out may be null; finished needs an eos_token in
  * [0, vocab), else it may be -1.  Outputs may not overlap inputs.
- * beams, n_out <= 128. */
+ * beams, n_out <= 128.  A workspace for a batch serves any smaller one (of the
+ * same beams, vocab and n_out), as sequences end. */
 typedef struct llmoc_beam_desc {
   int32_t batch, beams, vocab, n_out, eos_token;
 } llmoc_beam_desc;

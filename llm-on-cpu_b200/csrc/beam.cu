@@ -718,18 +718,33 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const __grid_const
 // Slices of the vocabulary per row, of at least eight tiles (one a warp): the
 // number that makes rounds of resident CTAs x (tiles a warp walks + what a CTA
 // costs besides, about five tiles) the smallest.
+static unsigned beam_tiles(int vocab, int f32) { return ((unsigned)vocab + (f32 ? 511 : 1023)) / (f32 ? 512 : 1024); }
 int beam_splits(int batch, int beams, int vocab, int f32) {
-  const unsigned rows = (unsigned)(batch * beams), tiles = ((unsigned)vocab + (f32 ? 511 : 1023)) / (f32 ? 512 : 1024);
+  const unsigned rows = (unsigned)(batch * beams), tiles = beam_tiles(vocab, f32);
   constexpr unsigned resident = 148 * 4;
   const unsigned most = std::min(std::max(1u, tiles / kRowWarps), 2 * resident);
   unsigned best = 1;
   unsigned long long cost = ~0ull;
   for (unsigned s = 1; s <= most; ++s) {
+    // no s from here on costs less than rows * s / resident x (tiles / (8 s) + 5)
+    if (rows * (tiles + 5ull * kRowWarps * s) / (resident * kRowWarps) >= cost) break;
     const unsigned per = (tiles + s * kRowWarps - 1) / (s * kRowWarps);
     const unsigned long long c = ((unsigned long long)rows * s + resident - 1) / resident * (per + 5);
     if (c < cost) best = s, cost = c;
   }
   return (int)best;
+}
+
+// The most lists (rows x slices) of any batch up to the given one: more rows may
+// take fewer slices in all.  From 148 (tiles / 8 + 5) rows on one slice a row is
+// the cheapest (a second costs rows / 592 x 4 more, the round it may save tiles /
+// 8 + 5), and the lists grow with the rows.
+long long beam_lists(int batch, int beams, int vocab, int f32) {
+  const long long one = 148ll * ((beam_tiles(vocab, f32) + kRowWarps - 1) / kRowWarps + 5);
+  long long most = (long long)batch * beams * beam_splits(batch, beams, vocab, f32);
+  for (int b = 1; b < batch && (long long)b * beams <= one; ++b)
+    most = std::max(most, (long long)b * beams * beam_splits(b, beams, vocab, f32));
+  return most;
 }
 
 cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t st) {

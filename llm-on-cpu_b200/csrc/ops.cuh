@@ -88,6 +88,7 @@ struct BeamArgs {
 constexpr int kBeamMaxOut = 128;
 constexpr int kBeamMaxBeams = 128;
 int beam_splits(int batch, int beams, int vocab, int f32);
+long long beam_lists(int batch, int beams, int vocab, int f32);
 cudaError_t launch_beam_select(const BeamArgs& a, cudaStream_t st);
 
 struct ReorderTensor {

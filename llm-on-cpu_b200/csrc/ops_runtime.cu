@@ -475,16 +475,13 @@ static llmoc_status check_beam(const llmoc_beam_desc* d, const char* who) {
   return LLMOC_OK;
 }
 
-// the workspace of a checked description; splits: slices per row of bf16 and of fp32 logits
-static size_t beam_bytes(const llmoc_beam_desc* d, int (&splits)[2]) {
-  for (int f32 = 0; f32 < 2; ++f32) splits[f32] = beam_splits(d->batch, d->beams, d->vocab, f32);
-  const size_t lists = (size_t)d->batch * d->beams * std::max(splits[0], splits[1]);
-  return up256(lists * d->n_out * 8) + up256(lists * 8);
+static size_t beam_bytes(const llmoc_beam_desc* d, long long lists) {
+  return up256((size_t)lists * d->n_out * 8) + up256((size_t)lists * 8);
 }
 
 size_t llmoc_beam_workspace_bytes(const llmoc_beam_desc* d) {
-  int splits[2];
-  return check_beam(d, "llmoc_beam_workspace_bytes") == LLMOC_OK ? beam_bytes(d, splits) : 0;
+  if (check_beam(d, "llmoc_beam_workspace_bytes") != LLMOC_OK) return 0;
+  return beam_bytes(d, std::max(beam_lists(d->batch, d->beams, d->vocab, 0), beam_lists(d->batch, d->beams, d->vocab, 1)));
 }
 
 llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int64_t ld, int logits_dtype,
@@ -518,8 +515,8 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
     for (int i = 0; i < o; ++i)
       if (overlap(outs[o], outs[i])) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": two outputs overlap");
   }
-  int splits[2];
-  const size_t need = beam_bytes(d, splits);
+  const int f32 = logits_dtype == LLMOC_DTYPE_F32, splits = beam_splits(d->batch, d->beams, d->vocab, f32);
+  const size_t need = beam_bytes(d, rows * splits);
   if (!workspace || workspace_bytes < need)
     return refuse(LLMOC_ERR_WORKSPACE, std::string(who) + ": workspace too small");
   if (!aligned(workspace, 8)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace is not aligned to 8");
@@ -533,7 +530,7 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
   BeamArgs a{};
   a.logits = logits;
   a.ld = ld;
-  a.f32 = logits_dtype == LLMOC_DTYPE_F32;
+  a.f32 = f32;
   a.scores = scores;
   a.fin = finished;
   a.batch = d->batch;
@@ -545,7 +542,7 @@ llmoc_status llmoc_beam_select(const llmoc_beam_desc* d, const void* logits, int
   a.token = token;
   a.out = out_scores;
   a.fin_out = finished_out;
-  a.splits = splits[a.f32];
+  a.splits = splits;
   a.vec = vec_rows(logits, ld * (long long)es);
   const size_t lists = (size_t)rows * a.splits;
   a.cand = (float2*)workspace;

@@ -184,3 +184,33 @@ def test_linear_status_refuses_a_null_handle():
 @pytest.mark.parametrize("ws", [A, 2 * A, 3 * A, 4 * A, 5 * A])
 def test_beam_workspace_apart_from_operands(ws):
     assert select(beam(), ws=ws) == 1 and "workspace overlaps" in L.last_error()
+
+
+@pytest.mark.parametrize("beams,vocab", [(1, 500), (4, 32003), (8, 32003), (4, 248320), (8, 248320), (5, 131072),
+                                         (128, 70001), (1, 1 << 20), (3, 8192)])
+def test_beam_workspace_of_a_batch_serves_smaller_ones(beams, vocab):
+    """As sequences end, calls with fewer of them take the workspace that the
+    largest batch asked for, with logits of either type."""
+    far = 1 << 50
+    sizes = [lib.llmoc_beam_workspace_bytes(C.byref(beam(batch=b, beams=beams, vocab=vocab))) for b in range(1, 201)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    big = [1 << i for i in range(8, 25 - beams.bit_length())]
+    more = [lib.llmoc_beam_workspace_bytes(C.byref(beam(batch=b, beams=beams, vocab=vocab))) for b in big]
+    assert [sizes[-1], *more] == sorted([sizes[-1], *more])
+    for dtype in (0, 1):
+        for top in (10, 25, 120, 200):
+            for b in range(1, top + 1):
+                # passes every check and stops at the device, which no machine has
+                d = beam(batch=b, beams=beams, vocab=vocab)
+                code = select(d, ld=vocab, dtype=dtype, logits=far, scores=2 * far, parent=3 * far, token=4 * far,
+                              out=5 * far, fin_out=6 * far, ws=7 * far, ws_bytes=sizes[top - 1], device=1 << 20)
+                assert code == 2, (b, top, L.last_error())
+
+
+def test_beam_workspace_of_the_largest_description():
+    """The size is found without walking through millions of batches at length."""
+    import time
+
+    t = time.monotonic()
+    assert lib.llmoc_beam_workspace_bytes(C.byref(beam(batch=1 << 24, beams=1, vocab=1 << 30, n_out=128))) > 1 << 34
+    assert time.monotonic() - t < 20
