@@ -409,6 +409,18 @@ def _device(x, device: int, what: str) -> int:
     return x.data_ptr()
 
 
+def _workspace(ws, ws_bytes: int, device: int):
+    """The address of a workspace: ws_bytes of a contiguous tensor on
+    cuda:`device`, or a raw device address."""
+    if ws is None or isinstance(ws, int):
+        return ws
+    if ws.get_device() != device:
+        raise LlmocError(f"the workspace is on {ws.device}, not on cuda:{device}")
+    if not ws.is_contiguous() or ws.numel() * ws.element_size() < ws_bytes:
+        raise LlmocError(f"the workspace is no contiguous tensor of {ws_bytes} bytes")
+    return ws.data_ptr()
+
+
 def _rows(x, rows: int, cols: int, device: int, what: str):
     """(address, row stride) of a [>= rows, cols] tensor with adjacent columns."""
     shape, stride = x.shape, x.stride()
@@ -574,8 +586,8 @@ class BeamSearch:
             None if finished is None else self._plain(finished, rows, 2, "finished"),
             self._plain(parent, kept, 1, "parent"), self._plain(token, kept, 1, "token"),
             self._plain(out_scores, kept, 0, "out_scores"),
-            None if finished_out is None else self._plain(finished_out, kept, 2, "finished_out"), ptr(ws), ws_bytes,
-            self.device, stream_ptr(stream))
+            None if finished_out is None else self._plain(finished_out, kept, 2, "finished_out"),
+            _workspace(ws, ws_bytes, self.device), ws_bytes, self.device, stream_ptr(stream))
         if st:
             check(st, "llmoc_beam_select")
 

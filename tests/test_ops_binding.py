@@ -1,0 +1,46 @@
+"""What the binding of the operators around the MoE layer refuses by itself, on a
+CPU-only host: an operator of "cuda:-1" takes CPU tensors as its own, and the
+library turns every call that reaches it down for the missing device."""
+import pytest
+
+import llmoc_b200 as L
+
+torch = pytest.importorskip("torch")
+
+
+class Elsewhere:
+    """A tensor on another device."""
+
+    def __init__(self, t, device):
+        self.t, self.index = t, device
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    @property
+    def device(self):
+        return torch.device("cuda", self.index)
+
+    def get_device(self):
+        return self.index
+
+
+def select(ws, ws_bytes):
+    bs = L.BeamSearch(1, 4, 64, 4, device=-1)
+    i = torch.zeros((1, 4), dtype=torch.int32)
+    bs.select(torch.zeros((4, 64)), torch.zeros((1, 4)), i, i.clone(), torch.zeros((1, 4)), ws, ws_bytes)
+
+
+def test_selection_checks_its_workspace():
+    n = L.BeamSearch(1, 4, 64, 4).workspace_bytes()
+    ws = torch.empty((n,), dtype=torch.uint8)
+    for good in (ws, torch.empty((n // 4,)), ws.data_ptr()):  # stop at the device
+        with pytest.raises(L.LlmocError, match="no such CUDA device"):
+            select(good, n)
+    with pytest.raises(L.LlmocError, match="workspace is on cuda:1"):
+        select(Elsewhere(ws, 1), n)
+    for bad in (ws[:-1], torch.empty((2 * n,), dtype=torch.uint8)[::2]):
+        with pytest.raises(L.LlmocError, match="workspace is no contiguous"):
+            select(bad, n)
+    with pytest.raises(L.LlmocError, match="workspace too small"):
+        select(ws[:-1], n - 1)
