@@ -243,9 +243,10 @@ def view_of(w) -> Int4View:
 class MoeLayer:
     """A device-resident MoE layer (llmoc_moe_layer_*)."""
 
-    def __init__(self, handle: int, desc: LayerDesc):
+    def __init__(self, handle: int, desc: LayerDesc, device: int = 0):
         self.handle = handle
         self.desc = desc
+        self.device = device
 
     @classmethod
     def create(cls, desc: LayerDesc, router_w, bias, experts: Sequence[Int4View],
@@ -257,7 +258,7 @@ class MoeLayer:
         fn = lib.llmoc_moe_layer_create_device if on_device else lib.llmoc_moe_layer_create
         check(fn(C.byref(desc), ptr(router_w), ptr(bias), arr, sh, device, C.byref(h)),
               "llmoc_moe_layer_create")
-        return cls(h.value, desc)
+        return cls(h.value, desc, device)
 
     @classmethod
     def from_host(cls, layer, device: int = 0) -> "MoeLayer":
@@ -283,7 +284,7 @@ class MoeLayer:
         h = C.c_void_p()
         check(lib.llmoc_moe_layer_create_qlwc(path.encode(), prefix.encode(), layer, C.byref(desc), device,
                                               C.byref(h)), "llmoc_moe_layer_create_qlwc")
-        return cls(h.value, desc)
+        return cls(h.value, desc, device)
 
     def set_shared_gate(self, gate_row, on_device: bool = False) -> None:
         """Per-token shared-expert weight sigmoid(gate_row . x) (bf16 [hidden])."""
@@ -331,9 +332,13 @@ class MoeLayer:
                       ws, ws_bytes: int, gate=None, stream=None) -> None:
         """The MoE block on its residual stream: before's pre norm, the layer,
         then after's post norm, gate, scales, residual add and pre norm."""
+        for norm in (before, after):
+            if norm.device != self.device:
+                raise LlmocError(f"llmoc_moe_forward_block: a norm on cuda:{norm.device}, the layer on cuda:{self.device}")
         io = after.io(T, None, residual, residual_out, norm_out, gate)
         check(lib.llmoc_moe_forward_block(self.handle, C.byref(before.desc), C.byref(after.desc), io, T,
-                                          ptr(ws), ws_bytes, stream_ptr(stream)), "llmoc_moe_forward_block")
+                                          _workspace(ws, ws_bytes, self.device), ws_bytes, stream_ptr(stream)),
+              "llmoc_moe_forward_block")
 
     def route(self, X, T: int, ws, ws_bytes: int, stream=None) -> None:
         check(lib.llmoc_moe_route(self.handle, ptr(X), T, ptr(ws), ws_bytes, stream_ptr(stream)),
@@ -654,8 +659,8 @@ class EpLayerShard(MoeLayer):
     """One rank's shard of an expert-parallel layer (llmoc_moe_layer_create_ep):
     routed experts e with e % world == rank, plus the router and shared expert."""
 
-    def __init__(self, handle: int, desc: LayerDesc, rank: int, world: int):
-        super().__init__(handle, desc)
+    def __init__(self, handle: int, desc: LayerDesc, rank: int, world: int, device: int = 0):
+        super().__init__(handle, desc, device)
         self.rank, self.world = rank, world
 
     @classmethod
@@ -668,7 +673,7 @@ class EpLayerShard(MoeLayer):
         h = C.c_void_p()
         check(lib.llmoc_moe_layer_create_ep(C.byref(desc), ptr(router_w), ptr(bias), arr, sh, device, rank, world,
                                             1 if on_device else 0, C.byref(h)), "llmoc_moe_layer_create_ep")
-        return cls(h.value, desc, rank, world)
+        return cls(h.value, desc, rank, world, device)
 
     @classmethod
     def from_host_ep(cls, layer, rank: int, world: int, device: int = 0) -> "EpLayerShard":

@@ -44,3 +44,25 @@ def test_selection_checks_its_workspace():
             select(bad, n)
     with pytest.raises(L.LlmocError, match="workspace too small"):
         select(ws[:-1], n - 1)
+
+
+def test_moe_block_checks_its_norms_and_workspace():
+    """The layer has no handle: what reaches the library is turned down there."""
+    layer = L.MoeLayer(None, None, device=-1)
+    here, there = L.ResidualNorm(64, pre="rms", device=-1), L.ResidualNorm(64, pre="rms", device=1)
+    x = torch.zeros((4, 64), dtype=torch.bfloat16)
+    ws = torch.empty((1 << 16,), dtype=torch.uint8)
+
+    def block(before, after, ws, ws_bytes):
+        layer.forward_block(before, after, 4, x, x.clone(), x.clone(), ws, ws_bytes)
+
+    for good in (ws, ws.data_ptr()):
+        with pytest.raises(L.LlmocError, match="bad arguments"):
+            block(here, here, good, ws.numel())
+    for norms in ((there, here), (here, there), (there, there)):
+        with pytest.raises(L.LlmocError, match="a norm on cuda:1"):
+            block(*norms, ws, ws.numel())
+    with pytest.raises(L.LlmocError, match="workspace is on cuda:1"):
+        block(here, here, Elsewhere(ws, 1), ws.numel())
+    with pytest.raises(L.LlmocError, match="workspace is no contiguous"):
+        block(here, here, ws, ws.numel() + 1)
