@@ -401,7 +401,8 @@ LLMOC_API llmoc_status llmoc_norm_residual(const llmoc_norm_desc* desc, const ll
  * `in` uses its pre norm only (its block, gate and scales are not applied);
  * out is the block's own post norm, scales and next norm; io gives residual,
  * residual_out, norm_out and gate (block is taken from the MoE layer, and the
- * dtypes of residual and norm_out must be bf16).  residual_out may be residual. */
+ * dtypes of residual and norm_out must be bf16).  residual_out may be residual.
+ * The workspace is aligned to 16 bytes and apart from io's operands. */
 LLMOC_API size_t llmoc_moe_block_workspace_bytes(const llmoc_moe_layer* layer, int max_tokens);
 LLMOC_API llmoc_status llmoc_moe_forward_block(const llmoc_moe_layer* layer, const llmoc_norm_desc* in,
                                                const llmoc_norm_desc* out, const llmoc_norm_io* io, int T,

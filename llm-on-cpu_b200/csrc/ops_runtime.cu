@@ -434,8 +434,11 @@ llmoc_status llmoc_moe_forward_block(const llmoc_moe_layer* layer, const llmoc_n
   if (!io->residual) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": null residual");
   if (io->residual_dtype != LLMOC_DTYPE_BF16 || (io->norm_out && io->norm_dtype != LLMOC_DTYPE_BF16))
     return refuse(LLMOC_ERR_INVALID, std::string(who) + ": residual and norm_out must be bf16");
-  if (!workspace || workspace_bytes < llmoc_moe_block_workspace_bytes(layer, T))
+  const size_t need = llmoc_moe_block_workspace_bytes(layer, T);
+  if (!workspace || workspace_bytes < need)
     return refuse(LLMOC_ERR_WORKSPACE, std::string(who) + ": workspace too small");
+  if (!aligned(workspace, 16))
+    return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace is not aligned to 16");
   char* x = (char*)workspace;
   char* b = x + up256((size_t)T * H * 2);
   char* ws = b + up256((size_t)T * H * 2);
@@ -454,7 +457,16 @@ llmoc_status llmoc_moe_forward_block(const llmoc_moe_layer* layer, const llmoc_n
   i2.block_dtype = LLMOC_DTYPE_BF16;
   const int dev = layer_device(layer);
   rc = norm_call(out, &i2, T, dev, stream, false);  // refuse before anything runs
-  if (rc == LLMOC_OK) rc = norm_call(&first, &i1, T, dev, stream, true);
+  if (rc != LLMOC_OK) return rc;
+  const long long gs = (long long)dtype_bytes(io->gate_dtype);
+  const Rows wr{workspace, (long long)need, (long long)need, 1};
+  for (const Rows& r : {Rows{io->residual, io->ld_residual * 2, H * 2ll, T},
+                        Rows{io->residual_out, io->ld_residual_out * 2, H * 2ll, T},
+                        Rows{io->norm_out, io->ld_norm_out * 2, H * 2ll, T},
+                        Rows{io->gate, io->gate_row_stride * gs, (io->gate_col_stride ? H : 1) * gs,
+                             io->gate_row_stride ? T : 1}})
+    if (overlap(wr, r)) return refuse(LLMOC_ERR_INVALID, std::string(who) + ": the workspace overlaps an operand");
+  rc = norm_call(&first, &i1, T, dev, stream, true);
   if (rc != LLMOC_OK) return rc;
   rc = llmoc_moe_forward(layer, (const uint16_t*)x, T, (uint16_t*)b, ws,
                          workspace_bytes - (size_t)(ws - (char*)workspace), stream);

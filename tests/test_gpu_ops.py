@@ -1096,3 +1096,30 @@ def test_select_mostly_masked_takes_no_longer():
             b.synchronize()
             times[masked].append(a.elapsed_time(b))
     assert float(np.median(times[True][2:])) < 2 * float(np.median(times[False][2:]))
+
+
+def test_moe_block_refuses_a_workspace_among_its_operands(oracle):
+    """A workspace that an operand shares, or that wide loads could not start in,
+    is refused before anything runs."""
+    layer = moe_layer(oracle)
+    H, T = 512, 6
+    before, after = L.ResidualNorm(H, pre="rms"), L.ResidualNorm(H, pre="rms")
+    n = layer.block_workspace_bytes(T)
+    whole = torch.zeros((n + 16 + T * H * 2,), dtype=torch.uint8, device="cuda")
+    ws = whole[:n]
+    at_end = whole[n - 16:n - 16 + T * H * 2].view(BF16).view(T, H)
+    at_start = whole[:T * H * 2].view(BF16).view(T, H)
+    r = torch.full((T, H), 3.0, dtype=BF16, device="cuda")
+    ro, no = torch.full_like(r, 5), torch.full_like(r, 7)
+    for x in (at_start, at_end):
+        for args, gate in (((x, ro, no), None), ((r, x, no), None), ((r, ro, x), None), ((r, ro, no), x),
+                           ((r, ro, no), x[:1]), ((r, ro, no), x[:, :1])):
+            with pytest.raises(L.LlmocError, match="workspace overlaps"):
+                layer.forward_block(before, after, T, *args, ws, n, gate=gate, stream=stream())
+    with pytest.raises(L.LlmocError, match="not aligned"):
+        layer.forward_block(before, after, T, r, ro, no, whole[8:n + 8], n, stream=stream())
+    torch.cuda.synchronize()
+    assert bool((whole == 0).all()) and bool((r == 3).all()) and bool((ro == 5).all()) and bool((no == 7).all())
+    layer.forward_block(before, after, T, r, ro, whole[n:n + T * H * 2].view(BF16).view(T, H), ws, n, stream=stream())
+    torch.cuda.synchronize()
+    layer.close()
