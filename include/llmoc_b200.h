@@ -443,7 +443,7 @@ LLMOC_API llmoc_status llmoc_beam_select(const llmoc_beam_desc* desc, const void
  * [0, beams) (e.g. -1) are left as they were, as is what lies between
  * segments.  A tensor may be reordered in place (dst == src, same strides,
  * n_out == beams): rows that stay are not touched.  Otherwise dst overlaps no
- * src (LLMOC_ERR_INVALID).  n_out <= 64.  The tensors' addresses are taken
+ * src (LLMOC_ERR_INVALID), nor parent.  n_out <= 64.  The tensors' addresses are taken
  * when the call is made; parent is read on the device. */
 typedef struct llmoc_reorder_tensor {
   const void* src;

@@ -597,10 +597,11 @@ llmoc_status llmoc_beam_reorder(const llmoc_reorder_tensor* tensors, int n_tenso
     int tensor;
     bool dst;
   };
-  Range few[2 * kReorderBatch];
-  Range* rg = n_tensors <= kReorderBatch ? few : new (std::nothrow) Range[2 * (size_t)n_tensors];
+  Range few[2 * kReorderBatch + 1];
+  Range* rg = n_tensors <= kReorderBatch ? few : new (std::nothrow) Range[2 * (size_t)n_tensors + 1];
   if (!rg) return refuse(LLMOC_ERR_NO_MEMORY, std::string(who) + ": out of memory");
   size_t nr = 0;
+  rg[nr++] = Range{(const char*)parent, (const char*)(parent + (size_t)batch * n_out), -1, false};
   for (int i = 0; i < n_tensors; ++i) {
     const llmoc_reorder_tensor& t = tensors[i];
     bool ok;
@@ -615,16 +616,18 @@ llmoc_status llmoc_beam_reorder(const llmoc_reorder_tensor* tensors, int n_tenso
   }
   std::sort(rg, rg + nr, [](const Range& a, const Range& b) { return a.lo < b.lo; });
   const char *any_end = nullptr, *dst_end = nullptr;
-  int bad = -1;
-  for (size_t i = 0; i < nr && bad < 0; ++i) {
-    if ((rg[i].dst ? any_end : dst_end) > rg[i].lo) bad = rg[i].tensor;
+  const Range* bad = nullptr;
+  for (size_t i = 0; i < nr && !bad; ++i) {
+    if ((rg[i].dst ? any_end : dst_end) > rg[i].lo) bad = rg + i;
     any_end = std::max(any_end, rg[i].hi);
     if (rg[i].dst) dst_end = std::max(dst_end, rg[i].hi);
   }
+  const int which = bad ? bad->tensor : 0;
   if (rg != few) delete[] rg;
-  if (bad >= 0)
-    return refuse(LLMOC_ERR_INVALID, std::string(who) + ": a destination overlaps a source or another destination (tensor " +
-                                         std::to_string(bad) + ")");
+  if (bad)
+    return refuse(LLMOC_ERR_INVALID,
+                  std::string(who) + ": a destination overlaps a source, another destination or parent (" +
+                      (which < 0 ? std::string("parent") : "tensor " + std::to_string(which)) + ")");
   OnDevice od(device);
   if (!od.ok) return no_device(who, device);
   for (int i0 = 0; i0 < n_tensors; i0 += kReorderBatch) {

@@ -214,3 +214,13 @@ def test_beam_workspace_of_the_largest_description():
     t = time.monotonic()
     assert lib.llmoc_beam_workspace_bytes(C.byref(beam(batch=1 << 24, beams=1, vocab=1 << 30, n_out=128))) > 1 << 34
     assert time.monotonic() - t < 20
+
+
+@pytest.mark.parametrize("parent", [2 * A, 2 * A + 508, 2 * A - 28])
+@pytest.mark.parametrize("n", [1, 60])
+def test_reorder_refuses_a_parent_in_a_destination(parent, n):
+    """The parents are read by every block, also after others have written."""
+    ts = (L.ReorderTensor * n)(*[tensor(src=(100 + 2 * i) * A, dst=(2 + 300 * i) * A) for i in range(n)])
+    assert lib.llmoc_beam_reorder(ts, n, parent, 2, 4, 4, 0, None) == 1 and "parent" in L.last_error()
+    assert lib.llmoc_beam_reorder(ts, n, 2 * A - 32, 2, 4, 4, 1 << 20, None) == 2  # beside it: only the device is missing
+    assert lib.llmoc_beam_reorder(ts, n, ts[0].src, 2, 4, 4, 1 << 20, None) == 2
