@@ -371,7 +371,12 @@ static llmoc_status norm_call(const llmoc_norm_desc* d, const llmoc_norm_io* io,
     if (overlap(g, range(2)) || overlap(g, range(3)))
       return refuse(LLMOC_ERR_INVALID, std::string(who) + ": an output overlaps the gate");
   }
-  for (const void* p : {d->post_weight, d->post_bias, d->pre_weight, d->pre_bias}) vec = vec && vec_rows(p, 0);
+  for (const void* p : {d->post_weight, d->post_bias, d->pre_weight, d->pre_bias}) {
+    const Rows w{p, 0, H * (long long)dtype_bytes(d->weight_dtype), 1};  // read anew for every row
+    if (overlap(w, range(2)) || overlap(w, range(3)))
+      return refuse(LLMOC_ERR_INVALID, std::string(who) + ": an output overlaps a weight");
+    vec = vec && vec_rows(p, 0);
+  }
   if (!run) return LLMOC_OK;
   OnDevice od(device);
   if (!od.ok) return no_device(who, device);

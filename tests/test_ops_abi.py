@@ -224,3 +224,15 @@ def test_reorder_refuses_a_parent_in_a_destination(parent, n):
     assert lib.llmoc_beam_reorder(ts, n, parent, 2, 4, 4, 0, None) == 1 and "parent" in L.last_error()
     assert lib.llmoc_beam_reorder(ts, n, 2 * A - 32, 2, 4, 4, 1 << 20, None) == 2  # beside it: only the device is missing
     assert lib.llmoc_beam_reorder(ts, n, ts[0].src, 2, 4, 4, 1 << 20, None) == 2
+
+
+@pytest.mark.parametrize("kw", [dict(norm_out=A), dict(residual_out=2 * A + 126), dict(norm_out=3 * A - 510),
+                                dict(residual_out=2 * A, ld_residual_out=72)])
+def test_norm_refuses_outputs_over_weights(kw):
+    assert lib.llmoc_norm_residual(C.byref(norm_desc()), C.byref(norm_io(**kw)), 4, 0, None) == 1, L.last_error()
+    assert "overlaps a weight" in L.last_error()
+
+
+def test_norm_takes_outputs_beside_weights():
+    for kw in (dict(norm_out=A + 128), dict(residual_out=2 * A - 512)):
+        assert lib.llmoc_norm_residual(C.byref(norm_desc()), C.byref(norm_io(**kw)), 4, 1 << 20, None) == 2
