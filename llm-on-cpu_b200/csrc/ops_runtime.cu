@@ -126,6 +126,9 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
     const int vgs = v.group_size > 0 ? v.group_size : 128, vzp = v.awq_zp > 0 ? v.awq_zp : 7;
     if (!v.qweight || !v.scales || v.M <= 0)
       return refuse(LLMOC_ERR_INVALID, std::string(who) + ": view " + std::to_string(i) + " is empty");
+    if (on_device && (!aligned(v.scales, 2) || (!awq && !aligned(v.zeros, 2))))
+      return refuse(LLMOC_ERR_INVALID,
+                    std::string(who) + ": view " + std::to_string(i) + ": a pointer is not aligned to its element");
     if (v.K != K || vgs != gs || v.scheme != scheme || (awq && vzp != zp))
       return refuse(LLMOC_ERR_INVALID, std::string(who) + ": view " + std::to_string(i) +
                                            " differs from the first in K, group size, scheme or zero point");
@@ -142,6 +145,17 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
   }
   OnDevice od(device);
   if (!od.ok) return no_device(who, device);
+  for (int i = 0; i < n_views && on_device; ++i)  // the kernel that packs them would fault on any other memory
+    for (const void* p : {(const void*)views[i].qweight, (const void*)views[i].scales,
+                          (const void*)(awq ? nullptr : views[i].zeros)}) {
+      cudaPointerAttributes at{};
+      if (!p) continue;
+      if (cudaPointerGetAttributes(&at, p) != cudaSuccess) cudaGetLastError();
+      if ((at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
+          (at.type == cudaMemoryTypeDevice && at.device != device))
+        return refuse(LLMOC_ERR_INVALID, std::string(who) + ": view " + std::to_string(i) + " is not in memory of device " +
+                                             std::to_string(device));
+    }
   auto* L = new (std::nothrow) llmoc_int4_linear();
   if (!L) return refuse(LLMOC_ERR_NO_MEMORY, std::string(who) + ": out of memory");
   L->device = device;

@@ -1123,3 +1123,18 @@ def test_moe_block_refuses_a_workspace_among_its_operands(oracle):
     layer.forward_block(before, after, T, r, ro, whole[n:n + T * H * 2].view(BF16).view(T, H), ws, n, stream=stream())
     torch.cuda.synchronize()
     layer.close()
+
+
+@pytest.mark.parametrize("asym", [False, True])
+def test_linear_create_refuses_host_memory_as_device_views(asym):
+    w = Weight(32, 64, 32, asym, seed=1)
+    host = [t.cpu() if t is not None else None for t in (w.q, w.s, w.z)]
+    dev = [w.q, w.s, w.z]
+    for i in range(3 if asym else 2):
+        v = [*dev[:i], host[i], *dev[i + 1:]]
+        view = L.view(*v, 32, 64, 32, L.SCHEME_GPTQ_ASYM if asym else L.SCHEME_AWQ_SYM)
+        with pytest.raises(L.LlmocError, match="not in memory of device 0"):
+            L.Int4Linear.create([w.view, view], on_device=True)
+    L.Int4Linear.create([w.view, w.view], on_device=True).close()
+    view = L.view(*host, 32, 64, 32, L.SCHEME_GPTQ_ASYM if asym else L.SCHEME_AWQ_SYM)
+    L.Int4Linear.create([view], on_device=False).close()

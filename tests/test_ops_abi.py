@@ -236,3 +236,12 @@ def test_norm_refuses_outputs_over_weights(kw):
 def test_norm_takes_outputs_beside_weights():
     for kw in (dict(norm_out=A + 128), dict(residual_out=2 * A - 512)):
         assert lib.llmoc_norm_residual(C.byref(norm_desc()), C.byref(norm_io(**kw)), 4, 1 << 20, None) == 2
+
+
+def test_linear_create_refuses_unaligned_scales():
+    """On the device they are read as they lie; host buffers are copied first."""
+    for kw in (dict(scales=2 * A + 1), dict(scheme=1, zeros=3 * A + 1)):
+        h = C.c_void_p()
+        assert lib.llmoc_int4_linear_create(views(**kw), 1, 1 << 20, 1, C.byref(h)) == 1 and "aligned" in L.last_error()
+        assert lib.llmoc_int4_linear_create(views(**kw), 1, 1 << 20, 0, C.byref(h)) == 2
+    assert lib.llmoc_int4_linear_create(views(zeros=3 * A + 1), 1, 1 << 20, 1, C.byref(h)) == 2  # not read
