@@ -384,13 +384,13 @@ cudaError_t launch_shape(const LinArgs& a, cudaStream_t st) {
   static_assert(2 * place + kLinWarps * NT * 8 * (16 + 4) * 4 + TP * 4 * 8 * 16 + 8 / FL * TP * 4 <= kLinSmemMax, "");
   const int smem = p.ring * place + p.bps * per_block + red;
   const auto kernel = k_linear<FL, AWQ, NT, TP>;
-  static bool attr[64] = {false};
+  static std::atomic<bool> attr[64];  // by device
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !attr[dev]) {
+  if (dev < 0 || dev >= 64 || !attr[dev].load(std::memory_order_relaxed)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmemMax);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) attr[dev] = true;
+    if (dev >= 0 && dev < 64) attr[dev].store(true, std::memory_order_relaxed);
   }
   const long long gx = ncl * (long long)c;
   if (gx > 0x7FFFFFFFll || ntb > 65535) return cudaErrorInvalidConfiguration;

@@ -68,6 +68,7 @@
 // drain warp gave back step j + 6's accumulator, which each does after it is
 // through with step j.
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <type_traits>
 
@@ -713,13 +714,13 @@ cudaError_t launch_u(const LinArgs& a, cudaStream_t st) {
   CUtensorMap xmap{};
   p.tma = a.x_vec && b_tensor_map(&xmap, a.X, a.K, a.T, a.ldx, p.N);
   const auto kernel = k_lin_umma<FL, AWQ>;
-  static bool attr[64] = {false};
+  static std::atomic<bool> attr[64];  // by device
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !attr[dev]) {
+  if (dev < 0 || dev >= 64 || !attr[dev].load(std::memory_order_relaxed)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) attr[dev] = true;
+    if (dev >= 0 && dev < 64) attr[dev].store(true, std::memory_order_relaxed);
   }
   const long long gx = (long long)((a.mt + 7) / 8) * p.c;
   if (gx > 0x7FFFFFFFll || ntb > 65535) return cudaErrorInvalidConfiguration;
