@@ -1138,3 +1138,37 @@ def test_linear_create_refuses_host_memory_as_device_views(asym):
     L.Int4Linear.create([w.view, w.view], on_device=True).close()
     view = L.view(*host, 32, 64, 32, L.SCHEME_GPTQ_ASYM if asym else L.SCHEME_AWQ_SYM)
     L.Int4Linear.create([view], on_device=False).close()
+
+
+@pytest.mark.parametrize("M,K,gs,T", [(20000, 6144, 128, 16), (20016, 6176, 32, 16), (20001, 6176, 64, 13),
+                                      (40000, 10240, 128, 8), (64, 99968, 128, 8)])
+@pytest.mark.parametrize("asym", [False, True])
+def test_linear_restages_activations(M, K, gs, T, asym):
+    """A CTA's share of K in more than one slab of staged activations: tile
+    groups after one another in a wide matrix, a split K in a long one."""
+    w = Weight(M, K, gs, asym, seed=M + K)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    for pad in (0, 3):
+        x = torch.randn((T, K + pad), generator=gen(T), device="cuda").to(BF16)[:, :K]
+        y = x.double() @ w.w.t()
+        got = run_linear(lin, w, x, T, F32)
+        close(got, y, w.tol(x, y, F32))
+        assert torch.equal(got, run_linear(lin, w, x, T, F32))
+    lin.status(stream())
+    lin.close()
+
+
+@pytest.mark.parametrize("M,K,gs,zp", [(300, 1408, 64, 7), (140, 992, 32, 7), (1000, 1024, 128, 7), (200, 640, 128, 20)])
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("T", [200, 512, 2049])
+def test_linear_of_a_prompt(M, K, gs, zp, asym, T):
+    w = Weight(M, K, gs, asym, seed=M + T, zp=zp)
+    lin = L.Int4Linear.create([w.view], on_device=True)
+    x = torch.randn((T, K), generator=gen(T), device="cuda").to(BF16)
+    r = torch.randn((T, M), generator=gen(T + 1), device="cuda").to(BF16)
+    y = x.double() @ w.w.t()
+    close(run_linear(lin, w, x, T, F32), y, w.tol(x, y, F32), "fp32")
+    yr = y + r.double()
+    close(run_linear(lin, w, x, T, BF16, R=r), yr, w.tol(x, yr, BF16) + 2 * U * (y.abs() + r.double().abs()), "bf16")
+    lin.status(stream())
+    lin.close()
