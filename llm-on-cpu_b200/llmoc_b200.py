@@ -619,10 +619,11 @@ class BeamReorder:
                 if not x.is_contiguous() or x.numel() % max(1, batch * rows):
                     raise LlmocError(f"BeamReorder: tensor {i} is not a contiguous block of {batch} x {rows} rows")
                 n[j] = x.numel() // max(1, batch * rows)
-            shape = tuple(s.shape[2:]) if s.dim() > 1 and tuple(s.shape[:2]) == (batch, beams) else tuple(s.shape[1:])
+            shape, to = [tuple(x.shape[2:]) if x.dim() > 1 and tuple(x.shape[:2]) == (batch, rows) else tuple(x.shape[1:])
+                         for x, rows in ((s, beams), (d, n_out))]
             if n[0] != n[1] or s.dtype != d.dtype:
                 raise LlmocError(f"BeamReorder: rows of tensor {i} differ in size or type")
-            self._row.append((shape, s.element_size(), n[0]))
+            self._row.append((shape, to, s.element_size(), n[0]))
             size = n[0] * s.element_size()
             self.tensors[i] = ReorderTensor(_device(s, device, f"src[{i}]"), _device(d, device, f"dst[{i}]"), size, size,
                                             0, size, 1)
@@ -631,9 +632,12 @@ class BeamReorder:
 
     def set_used(self, used: int) -> None:
         """Move only the first `used` indices of dimension `dim` of every row from now on."""
-        for i, (shape, es, n) in enumerate(self._row):
+        for i, (shape, to, _, _) in enumerate(self._row):
             if self.dim >= len(shape) or not 0 <= used <= shape[self.dim]:
                 raise LlmocError(f"BeamReorder: {used} of dimension {self.dim} of rows {shape}")
+            if shape != to:
+                raise LlmocError(f"BeamReorder: rows of tensor {i} differ in shape")
+        for i, (shape, _, es, n) in enumerate(self._row):
             inner = es
             for v in shape[self.dim + 1:]:
                 inner *= v

@@ -66,3 +66,23 @@ def test_moe_block_checks_its_norms_and_workspace():
         block(here, here, Elsewhere(ws, 1), ws.numel())
     with pytest.raises(L.LlmocError, match="workspace is no contiguous"):
         block(here, here, ws, ws.numel() + 1)
+
+
+def test_reorder_of_a_used_length_changes_all_tensors_or_none():
+    a, b = torch.zeros((2, 3, 10, 4)), torch.zeros((2, 3, 6, 4))
+    move = L.BeamReorder([a, b], [a.clone(), b.clone()], 2, 3, 3, device=-1, used=5)
+    want = [(t.n_seg, t.seg_stride, t.seg_bytes) for t in move.tensors]
+    assert want == [(1, 160, 80), (1, 96, 80)]
+    for used in (8, -1):  # more than b has
+        with pytest.raises(L.LlmocError, match=f"{used} of dimension 0"):
+            move.set_used(used)
+        assert [(t.n_seg, t.seg_stride, t.seg_bytes) for t in move.tensors] == want
+
+
+def test_reorder_of_a_used_length_needs_rows_of_one_shape():
+    """Rows of other dimensions hold the used part elsewhere; whole rows move as bytes."""
+    src, other = torch.zeros((2, 3, 10, 4)), torch.zeros((2, 3, 4, 10))
+    L.BeamReorder([src], [other], 2, 3, 3, device=-1)
+    L.BeamReorder([src], [torch.zeros((6, 10, 4))], 2, 3, 3, device=-1, dim=1, used=2)  # batch and beams in one
+    with pytest.raises(L.LlmocError, match="differ in shape"):
+        L.BeamReorder([src], [other], 2, 3, 3, device=-1, used=3)
