@@ -633,7 +633,7 @@ class BeamReorder:
     def set_used(self, used: int) -> None:
         """Move only the first `used` indices of dimension `dim` of every row from now on."""
         for i, (shape, to, _, _) in enumerate(self._row):
-            if self.dim >= len(shape) or not 0 <= used <= shape[self.dim]:
+            if not 0 <= self.dim < len(shape) or not 0 <= used <= shape[self.dim]:
                 raise LlmocError(f"BeamReorder: {used} of dimension {self.dim} of rows {shape}")
             if shape != to:
                 raise LlmocError(f"BeamReorder: rows of tensor {i} differ in shape")

@@ -86,3 +86,11 @@ def test_reorder_of_a_used_length_needs_rows_of_one_shape():
     L.BeamReorder([src], [torch.zeros((6, 10, 4))], 2, 3, 3, device=-1, dim=1, used=2)  # batch and beams in one
     with pytest.raises(L.LlmocError, match="differ in shape"):
         L.BeamReorder([src], [other], 2, 3, 3, device=-1, used=3)
+
+
+def test_reorder_refuses_a_dimension_counted_from_the_end():
+    """Taken as it is, it would put the end of a row's segment past the row."""
+    src = torch.zeros((1, 1, 4, 8))
+    for dim in (-1, -2, 2):
+        with pytest.raises(L.LlmocError, match=f"dimension {dim}"):
+            L.BeamReorder([src], [src.clone()], 1, 1, 1, device=-1, dim=dim, used=3)
