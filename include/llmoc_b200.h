@@ -331,13 +331,15 @@ enum { LLMOC_ACT_NONE = 0, LLMOC_ACT_SIGMOID = 1 };
  * M = sum of their rows; they agree in K, group size, scheme and zero point, and
  * every one but the last has a multiple of 16 rows.  K and the group size are
  * multiples of 32 (LLMOC_ERR_UNSUPPORTED otherwise); M is any.  on_device: the
- * views point to memory of `device`, complete when the call is made.  The
- * views' buffers are not kept. */
+ * views point to memory of `device`, scales and zeros at even addresses
+ * (LLMOC_ERR_INVALID otherwise), complete when the call is made.  The views'
+ * buffers are not kept. */
 typedef struct llmoc_int4_linear llmoc_int4_linear;
 LLMOC_API llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views, int device, int on_device,
                                                 llmoc_int4_linear** out);
 LLMOC_API void llmoc_int4_linear_destroy(llmoc_int4_linear* linear);
-/* Bytes of resident weights one product streams (packed q + fp16 scales / zeros, with the padding to 16 rows x 64 k). */
+/* Bytes of resident weights one product streams (packed q + fp16 scales / zeros),
+ * with the padding to 16 rows x 256 k: K = 288 streams the bytes of 512. */
 LLMOC_API size_t llmoc_int4_linear_weight_bytes(const llmoc_int4_linear* linear);
 /* Y[t, m] = sum_k W[m, k] X[t, k] (+ R[t, m]), t < T, one rounding to y_dtype
  * (LLMOC_DTYPE_*): products of bf16 activations with exact integers (or, from 9
@@ -443,8 +445,10 @@ LLMOC_API llmoc_status llmoc_beam_select(const llmoc_beam_desc* desc, const void
  * [0, beams) (e.g. -1) are left as they were, as is what lies between
  * segments.  A tensor may be reordered in place (dst == src, same strides,
  * n_out == beams): rows that stay are not touched.  Otherwise dst overlaps no
- * src (LLMOC_ERR_INVALID), nor parent.  n_out <= 64.  The tensors' addresses are taken
- * when the call is made; parent is read on the device. */
+ * src (LLMOC_ERR_INVALID), nor parent.  n_out <= 64 (a selection may keep up to
+ * 128).  Rows move by accesses as wide as all addresses and strides allow, up to 16
+ * bytes; an odd one among them makes it single bytes.  The tensors' addresses are
+ * taken when the call is made; parent is read on the device. */
 typedef struct llmoc_reorder_tensor {
   const void* src;
   void* dst;

@@ -24,11 +24,15 @@
 //                 a bound, what reaches it, ranked by counting.
 //
 // What bounds it (graph replay): 32 sequences x 8 beams x 248320 bf16 logits take
-// 44.4 us, 2.9 TB/s; of those the exponentials alone, 4 a clock and scheduler, are
-// 14 us, and with the unpacking, sums and comparisons a scheduler needs some 360
-// cycles for a warp's 1024 elements.  Rows copied ahead in bulk were 3 % slower: it
-// does not wait for memory.  Nor does it gain from CTAs gathered on the live rows
-// when some are finished.  8 x 4 x 131072 fp32 with 8 candidates take 15.0 us
+// 44.4 us, 2.9 TB/s.  No unit is busy all of that time: the instructions, some 390 a
+// scheduler for a warp's 1024 elements, fill 21 us (the exponentials' unit 17 of
+// them), the bytes 20.  A fifth of the time an SM has no warp (the launch, the last
+// CTAs); in the rest a scheduler issues in 61 % of the cycles, since 512 CTAs on 592
+// places leave it six warps, each of which waits ten cycles per instruction: fixed
+// latencies 2.3, loads 1.4, barriers 1.0, instruction fetch and branches 1.1, its
+// turn 1.4.  With a fifth of the beams finished (the time is the same) it issues in
+// 54 %, and SMs differ by much.  Rows copied ahead in bulk were 3 % slower, and CTAs
+// gathered on the live rows gain nothing.  8 x 4 x 131072 fp32 with 8 candidates take 15.0 us
 // (1.1 TB/s), 1 x 4 x 32003 7.6 us, of which the two launches and a chain of load,
 // first bound, list and merge are nearly all; the merge has 3 to 5 us of each.
 //
@@ -213,7 +217,7 @@ __device__ __noinline__ int bisect_slice(const BeamArgs& a, long long base, int 
 // its first maximum, which moves only when a logit exceeds it by more than
 // kRefSlack.
 //
-// What is rare, a tile with a NaN or +inf, goes through one rolled loop that
+// What is rare, a tile with a NaN, +inf or values above kScaleMax, goes through one rolled loop that
 // reads the logits again and masks them (`careful`).  So the loop that runs hot
 // stays small: inlined per piece, these cases doubled the time by instruction
 // fetches alone.  Vocabularies of fewer
