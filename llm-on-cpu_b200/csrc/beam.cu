@@ -85,8 +85,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Above kScaleMax the products would leave fp32: exp(x - m) as 2^((x - m) * kLog2e).
-constexpr float kScaleMax = 1e38f;
+// At kScaleMax the rounding of the product is up to 16, a factor of 2^16 that the
+// sum can bear; above it exp(x - m) is 2^((x - m) * kLog2e), relative to m itself.
+// Logits of which one lies above it and one below are at least 32 apart: what such
+// a change of reference carries over is below 2^16 e^-32 of the sum, and not
+// corrected for.
+constexpr float kScaleMax = 0x1p28f;
 // the factor from a sum relative to m to one relative to n
 __device__ __forceinline__ float rescale(float m, float n) {
   return exp2_fast(fabsf(m) <= kScaleMax && fabsf(n) <= kScaleMax ? __fsub_rn(log2_ref(m), log2_ref(n)) : (m - n) * kLog2e);

@@ -1172,3 +1172,20 @@ def test_linear_of_a_prompt(M, K, gs, zp, asym, T):
     close(run_linear(lin, w, x, T, BF16, R=r), yr, w.tol(x, yr, BF16) + 2 * U * (y.abs() + r.double().abs()), "bf16")
     lin.status(stream())
     lin.close()
+
+
+@pytest.mark.parametrize("V", [60, 5000, 40001])
+@pytest.mark.parametrize("scale", [1e4, 1e6, 2.0 ** 24, 2.0 ** 27, 1e9, 1e15, 1e30, 1e38])
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_select_with_large_logits(V, scale, dt):
+    """Logits whose products with log2(e) round by far more than a bit, up to
+    those whose products leave fp32, of either sign, alone or among small ones."""
+    B, W, k = 3, 4, 5
+    g = gen(V)
+    x = torch.randn((B * W, V), generator=g, device="cuda")
+    few = torch.rand((B * W, V), generator=g, device="cuda") < 0.01
+    scores = -20 * torch.rand((B, W), generator=g, device="cuda")
+    near = 1 + torch.round(x * 4) * 2.0 ** -23  # a few neighbours of one value
+    for logits in (x * (scale / 8), -x.abs() * (scale / 8), torch.where(few, x * (scale / 8), x), near * scale,
+                   -near * scale):
+        check_select(logits.to(dt), scores, None, -1, k)
