@@ -414,8 +414,8 @@ LLMOC_API llmoc_status llmoc_moe_forward_block(const llmoc_moe_layer* layer, con
  * no reference counterpart).  logits [batch * beams][ld >= vocab], bf16 or
  * fp32; candidate (w, v) of sequence b has the value
  *     scores[b][w] + logit - log sum exp(logits of the beam),
- * and the n_out best over all beams and tokens, ordered by value, then beam,
- * then token, are written: parent (the beam), token, out_scores, all
+ * and the n_out best over all beams and tokens, ordered by value (in fp64), then
+ * beam, then token, are written: parent (the beam), token, out_scores, all
  * [batch][n_out].  Non-finite logits are masked: their tokens are no
  * candidates and add nothing to the sum.  A beam whose score is not finite has
  * no candidates (e.g. all but the first of a sequence's first step).  A beam
