@@ -145,14 +145,13 @@ llmoc_status llmoc_int4_linear_create(const llmoc_int4_view* views, int n_views,
   }
   OnDevice od(device);
   if (!od.ok) return no_device(who, device);
-  for (int i = 0; i < n_views && on_device; ++i)  // the kernel that packs them would fault on any other memory
+  for (int i = 0; i < n_views && on_device; ++i)  // the kernel that packs them would fault on pageable memory
     for (const void* p : {(const void*)views[i].qweight, (const void*)views[i].scales,
                           (const void*)(awq ? nullptr : views[i].zeros)}) {
       cudaPointerAttributes at{};
       if (!p) continue;
       if (cudaPointerGetAttributes(&at, p) != cudaSuccess) cudaGetLastError();
-      if ((at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
-          (at.type == cudaMemoryTypeDevice && at.device != device))
+      if (at.type == cudaMemoryTypeUnregistered || (at.type == cudaMemoryTypeDevice && at.device != device))
         return refuse(LLMOC_ERR_INVALID, std::string(who) + ": view " + std::to_string(i) + " is not in memory of device " +
                                              std::to_string(device));
     }

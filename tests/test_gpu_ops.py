@@ -1138,6 +1138,9 @@ def test_linear_create_refuses_host_memory_as_device_views(asym):
     L.Int4Linear.create([w.view, w.view], on_device=True).close()
     view = L.view(*host, 32, 64, 32, L.SCHEME_GPTQ_ASYM if asym else L.SCHEME_AWQ_SYM)
     L.Int4Linear.create([view], on_device=False).close()
+    pinned = [t.pin_memory() if t is not None else None for t in host]  # the device can read it
+    view = L.view(*pinned, 32, 64, 32, L.SCHEME_GPTQ_ASYM if asym else L.SCHEME_AWQ_SYM)
+    L.Int4Linear.create([view], on_device=True).close()
 
 
 @pytest.mark.parametrize("M,K,gs,T", [(20000, 6144, 128, 16), (20016, 6176, 32, 16), (20001, 6176, 64, 13),
